@@ -75,6 +75,16 @@ class ef_hip_reply_stats(C.Structure):
                 ("eos_p_max", C.c_double), ("eos_p_max_step", _sz)]
 
 
+class ef_hip_page_pool(C.Structure):
+    _fields_ = [("k_dev", _P), ("v_dev", _P), ("qtype", C.c_int)] + \
+               [(n, _sz) for n in ("n_pages", "page_size", "KV", "hd", "page_stride")]
+
+
+class ef_hip_paged_batch(C.Structure):
+    _fields_ = [(n, _P) for n in ("row_start_dev", "kv_len_dev", "table_dev")] + \
+               [(n, _sz) for n in ("table_ld", "n_seqs", "max_rows", "max_new", "max_kv")]
+
+
 STOP_NONE, STOP_EOS, STOP_EOS_MIN_P, STOP_MAX_NEW, STOP_CONTEXT = 0, 1, 2, 5, 6
 
 
@@ -150,6 +160,16 @@ SIGNATURES = {
     "ef_hip_compare_dist": (C.c_int, [_P, _P, _sz, _sz, _sz, _sz, C.POINTER(C.c_double), C.POINTER(ef_hip_dist_stats),
                                       _P]),
     "ef_hip_neg_log_prob": (C.c_int, [_P, _sz, _sz, _sz, _P, _P, _P]),
+    "ef_hip_page_plan": (C.c_int, [_P, _P, _sz, _sz, _sz, _P, _sz, _P, _P, _P, _P, _P, _P, _P, _sz, _P, _P]),
+    "ef_hip_rope_tables": (C.c_int, [C.c_float, _sz, _sz, _P, _P]),
+    "ef_hip_rope_append": (C.c_int, [_P, _sz, _P, _sz, _sz, _P, _sz, _P, _sz, _P, _sz, _sz, _P, _P, _P, _sz, _P,
+                                     C.POINTER(ef_hip_page_pool), _P]),
+    "ef_hip_paged_attention_workspace_bytes": (_sz, [_sz, C.POINTER(ef_hip_page_pool), _sz, _sz, _sz, _sz]),
+    "ef_hip_paged_attention": (C.c_int, [_P, _sz, _P, _sz, _sz, C.POINTER(ef_hip_page_pool),
+                                         C.POINTER(ef_hip_paged_batch), C.c_float, _P, _sz, _P]),
+    "ef_hip_packed_attention_workspace_bytes": (_sz, [_sz, _sz, _sz, C.c_int, _sz, _sz]),
+    "ef_hip_packed_attention": (C.c_int, [_P, _sz, _P, _sz, _P, _sz, C.c_int, _P, _sz, _sz, _sz, _sz, _P, _sz, _sz,
+                                          C.c_float, _P, _sz, _P]),
     "ef_hip_efq_open": (C.c_int, [C.c_char_p, C.POINTER(_P)]),
     "ef_hip_efq_parse": (C.c_int, [_P, _sz, C.POINTER(_P)]),
     "ef_hip_efq_close": (C.c_int, [_P]),

@@ -26,6 +26,7 @@
 #include "common.h"
 #include "gemv.h"
 #include "glue.h"
+#include "paging.h"
 #include "sampler.h"
 
 namespace {
@@ -774,21 +775,8 @@ int ef_hip_engine_create(const ef_hip_model_config* cfg, const ef_hip_layer* lay
   if (hipHostMalloc(reinterpret_cast<void**>(&e->stage), (B * S + 8) * sizeof(int32_t), hipHostMallocDefault) !=
       hipSuccess)
     return cleanup_fail(fail(EF_HIP_ENOMEM, "engine pinned staging"));
-  // RoPE tables exactly as kern::RopeTable builds them (src/kernels.cpp:113-131): float pow / cos /
-  // sin from the host C library, so the device sees the reference's bits.
-  const size_t half = c.hd / 2;
-  std::vector<float> inv(half), ct(S * half), st(S * half);
-  for (size_t i = 0; i < half; ++i) {
-    const float expo = static_cast<float>(2 * i) / static_cast<float>(c.hd);
-    inv[i] = 1.0f / std::pow(c.rope_theta, expo);
-  }
-  for (size_t p = 0; p < S; ++p) {
-    for (size_t i = 0; i < half; ++i) {
-      const float ang = static_cast<float>(p) * inv[i];
-      ct[p * half + i] = std::cos(ang);
-      st[p * half + i] = std::sin(ang);
-    }
-  }
+  std::vector<float> ct, st;
+  rope_tables_host(c.rope_theta, c.hd, S, &ct, &st);
   hipError_t he = hipMemcpyAsync(e->cos_t, ct.data(), ct.size() * 4, hipMemcpyHostToDevice, e->stream);
   if (he == hipSuccess) he = hipMemcpyAsync(e->sin_t, st.data(), st.size() * 4, hipMemcpyHostToDevice, e->stream);
   if (he == hipSuccess) he = hipMemsetAsync(e->kc, 0, c.L * B * S * kvd * 4, e->stream);

@@ -14,7 +14,8 @@ from ._lib import BF16, F16, F32, Q4_0, Q8_0, call, lib
 
 __all__ = ["DeviceArray", "Weight", "Stream", "Event", "init", "row_bytes", "matvec", "matvec_jobs",
            "matvec_residual", "matvec_swiglu", "matvec_jobs_rmsnorm", "quantize", "rows_f32", "argmax", "sampler_exp",
-           "RngStates", "sample", "F32", "F16", "BF16", "Q8_0", "Q4_0"]
+           "RngStates", "sample", "PagePool", "page_plan", "rope_tables", "rope_append", "paged_attention",
+           "paged_attention_workspace_bytes", "packed_attention", "packed_attention_workspace_bytes", "F32", "F16", "BF16", "Q8_0", "Q4_0"]
 
 
 def init(device: int = 0) -> None:
@@ -233,3 +234,75 @@ def sample(logits: DeviceArray, vocab: int, cfg: dict, out: DeviceArray, batch: 
     call("ef_hip_sample", logits.ptr, vocab, batch, ld or vocab, C.byref(c), hist.ptr if hist else None,
          hist_len.ptr if hist_len else None, hist_ld, rng.buf.ptr if rng else None, out.ptr,
          ws.ptr if ws else None, _s(stream))
+
+
+def _p(x):
+    """Device address of a DeviceArray (or of anything with .ptr), or of a raw one."""
+    return x if x is None or isinstance(x, int) else x.ptr
+
+
+class PagePool:
+    """A pool of KV pages (ef_hip_page_pool): n_pages pages of [KV][page_size][hd] values each of K and V,
+    in the caller's device memory (k, v) or in its own (zeros)."""
+
+    def __init__(self, n_pages: int, page_size: int, KV: int, hd: int, qtype: int = F32, k=None, v=None,
+                 page_stride: int = 0):
+        init()
+        if qtype not in (F32, F16, BF16):
+            raise ValueError("pages hold F32, F16 or BF16 values")
+        self.n_pages, self.page_size, self.KV, self.hd, self.qtype = n_pages, page_size, KV, hd, qtype
+        self.page_stride = page_stride or KV * page_size * hd
+        nbytes = n_pages * self.page_stride * (4 if qtype == F32 else 2)
+        own = []
+        for given in (k, v):
+            own.append(given if given is not None else DeviceArray((nbytes,), np.uint8))
+            if given is None:
+                own[-1].zero()
+        self.k, self.v = own
+        sync()
+        self.c = L.ef_hip_page_pool(_p(self.k), _p(self.v), qtype, n_pages, page_size, KV, hd, self.page_stride)
+
+
+def page_plan(cached, new, seqs: int, page_size: int, n_pages: int, table, table_ld: int, free, n_free, n_free_out, kv_len,
+              row_start, pos, slot, max_rows: int, status, stream=None) -> None:
+    """One step's block tables and slot maps from the requests' lengths (ef_hip_page_plan)."""
+    call("ef_hip_page_plan", _p(cached), _p(new), seqs, page_size, n_pages, _p(table), table_ld, _p(free), _p(n_free),
+         _p(n_free_out), _p(kv_len), _p(row_start), _p(pos), _p(slot), max_rows, _p(status), _s(stream))
+
+
+def rope_tables(theta: float, hd: int, n_pos: int) -> tuple[DeviceArray, DeviceArray]:
+    """cos and sin [n_pos][hd / 2] as the engine's (ef_hip_rope_tables)."""
+    cos, sin = DeviceArray((n_pos, hd // 2)), DeviceArray((n_pos, hd // 2))
+    call("ef_hip_rope_tables", theta, hd, n_pos, cos.ptr, sin.ptr)
+    return cos, sin
+
+
+def rope_append(q, ldq: int, q_out, ldqo: int, heads: int, k, ldk: int, v, ldv: int, rows: int, pos, cos, sin, n_pos: int,
+                slot, pool: PagePool, k_out=None, ldko: int = 0, stream=None) -> None:
+    """RoPE on queries and keys, keys and values stored into the pool (ef_hip_rope_append)."""
+    call("ef_hip_rope_append", _p(q), ldq, _p(q_out), ldqo, heads, _p(k), ldk, _p(k_out), ldko, _p(v), ldv, rows, _p(pos),
+         _p(cos), _p(sin), n_pos, _p(slot), C.byref(pool.c), _s(stream))
+
+
+def paged_attention_workspace_bytes(heads: int, pool: PagePool, seqs: int, max_rows: int, max_new: int,
+                                    max_kv: int) -> int:
+    return lib().ef_hip_paged_attention_workspace_bytes(heads, C.byref(pool.c), seqs, max_rows, max_new, max_kv)
+
+
+def paged_attention(q, ldq: int, out, ldo: int, heads: int, pool: PagePool, table, table_ld: int, row_start, kv_len,
+                    seqs: int, max_rows: int, max_new: int, max_kv: int, scale: float, ws=None, stream=None) -> None:
+    """Attention of each request's new rows over its pages (ef_hip_paged_attention)."""
+    b = L.ef_hip_paged_batch(_p(row_start), _p(kv_len), _p(table), table_ld, seqs, max_rows, max_new, max_kv)
+    call("ef_hip_paged_attention", _p(q), ldq, _p(out), ldo, heads, C.byref(pool.c), C.byref(b), scale, _p(ws),
+         ws.nbytes if ws is not None else 0, _s(stream))
+
+
+def packed_attention_workspace_bytes(heads: int, KV: int, hd: int, qtype: int, seqs: int, max_rows: int) -> int:
+    return lib().ef_hip_packed_attention_workspace_bytes(heads, KV, hd, qtype, seqs, max_rows)
+
+
+def packed_attention(q, ldq: int, k, ldk: int, v, ldv: int, qtype: int, out, ldo: int, heads: int, KV: int, hd: int, row_start,
+                     seqs: int, max_rows: int, scale: float, ws=None, stream=None) -> None:
+    """Causal attention over packed prompts (ef_hip_packed_attention)."""
+    call("ef_hip_packed_attention", _p(q), ldq, _p(k), ldk, _p(v), ldv, qtype, _p(out), ldo, heads, KV, hd, _p(row_start),
+         seqs, max_rows, scale, _p(ws), ws.nbytes if ws is not None else 0, _s(stream))

@@ -322,6 +322,95 @@ int ef_hip_engine_reset(ef_hip_engine e);
 int ef_hip_engine_score(ef_hip_engine e, const int32_t* ids_host, size_t n, size_t first, double* nll_host,
                         float* logits_dev);
 
+/* ---- paged serving ------------------------------------------------------------------------------
+ * No counterpart in the reference (one sequence, one contiguous cache): what a server of many
+ * requests of different lengths runs on.  The cache is a pool of pages of page_size positions each;
+ * a request's page b holds its positions b * page_size .. and its number stands in the block table,
+ * table_dev[r * table_ld + b].  Every call is stream-ordered, allocates nothing and reads the
+ * requests' lengths from device memory, so that a captured step serves every later one of the same
+ * bounds.  Calls that run at the same time need workspaces of their own.
+ *
+ * The pool: page p of K starts at k_dev + p * page_stride values of `qtype` (EF_QTYPE_F32, F16 or
+ * BF16) and holds [KV][page_size][hd]; V likewise.  page_size is a power of two up to 1024, hd a
+ * multiple of 8 up to 256, page_stride at least KV * page_size * hd (0: exactly that; larger where
+ * layers or K and V share their pages' memory), pages and addresses at multiples of 16 bytes. */
+typedef struct {
+  void *k_dev, *v_dev;
+  int qtype;
+  size_t n_pages, page_size, KV, hd, page_stride;
+} ef_hip_page_pool;
+
+/* One step's block tables and slot maps from the requests' lengths, on the device.
+ * Request r < n_seqs has cached_dev[r] positions in its pages and gets new_dev[r] more rows in this
+ * step (0: it waits; negative: it ended and gives its pages back).  free_dev[0 .. *n_free_dev) are
+ * the free pages' numbers, the last one taken first; the array has room for n_pages.
+ *  - The pages of ended requests (table entries in [0, n_pages)) are put on top of the free ones, in
+ *    order; their table rows keep their entries, which no length reaches any more.
+ *  - Growing requests take pages from the top, in order, into their table rows.
+ *  - row_start_dev[n_seqs + 1] gets the first row of each request (row_start_dev[n_seqs]: how many),
+ *    pos_dev / slot_dev[max_rows] each row's position and slot (page * page_size + offset; position
+ *    0 and slot -1 behind the last row), kv_len_dev[n_seqs] the positions after the step (0 for
+ *    ended requests), *n_free_out_dev the free pages left.
+ *  - status_dev[4]: pages that are missing, requests with a bad length (negative cached, or more
+ *    positions than table_ld pages hold), rows that do not fit max_rows, 1 for a free count outside
+ *    [0, n_pages].  All zero, or the step did not fit and nothing is taken or given back: the
+ *    table, the free pages and both lengths stay, row_start_dev is 0 and every slot -1, so
+ *    that the rest of a captured step finds no rows.
+ * kv_len_dev may be cached_dev and n_free_out_dev may be n_free_dev (in place). */
+int ef_hip_page_plan(const int32_t* cached_dev, const int32_t* new_dev, size_t n_seqs, size_t page_size, size_t n_pages,
+                     int32_t* table_dev, size_t table_ld, int32_t* free_dev, const int32_t* n_free_dev,
+                     int32_t* n_free_out_dev, int32_t* kv_len_dev, int32_t* row_start_dev, int32_t* pos_dev,
+                     int64_t* slot_dev, size_t max_rows, int32_t* status_dev, void* stream);
+
+/* cos / sin [n_pos][hd / 2] of RoPE as the engine's own tables (kern::RopeTable, src/kernels.cpp:113-131:
+ * float angles, the host C library's functions).  Synchronous. */
+int ef_hip_rope_tables(float theta, size_t hd, size_t n_pos, float* cos_dev, float* sin_dev);
+
+/* RoPE (half-split pairs, src/kernels.cpp:133-146) on `rows` rows of `heads` query heads and
+ * pool->KV key heads at positions pos_dev[rows], and the turned keys and the values stored into the
+ * pool at slot_dev[rows] (one rounding to the pool's type; a slot outside the pool stores nothing;
+ * the slots of a call that are in it differ).  q / k / v are FP32 rows with strides ldq / ldk / ldv in
+ * floats; q_out may be q_dev, k_out (optional: the turned keys in FP32) may be k_dev.  A row whose
+ * position is outside [0, n_pos) gets NaN and stores nothing.  Strides and addresses at multiples of 16
+ * bytes. */
+int ef_hip_rope_append(const float* q_dev, size_t ldq, float* q_out_dev, size_t ldqo, size_t heads, const float* k_dev,
+                       size_t ldk, float* k_out_dev, size_t ldko, const float* v_dev, size_t ldv, size_t rows,
+                       const int32_t* pos_dev, const float* cos_dev, const float* sin_dev, size_t n_pos,
+                       const int64_t* slot_dev, const ef_hip_page_pool* pool, void* stream);
+
+/* Attention of the requests' new rows over their pages: request r's rows row_start_dev[r] ..
+ * row_start_dev[r + 1] (n of them; row_start as ef_hip_page_plan leaves it, increasing) hold its last
+ * n positions, so row i sees positions 0 .. kv_len_dev[r] - n + i:
+ *   out = sum_j softmax_j(scale * q . k_j) v_j,  query head h over KV head h / (heads / KV).
+ * A page number outside [0, n_pages) is no page: its positions take no part.  A row that sees nothing
+ * gets zeros.  Rows behind row_start_dev[n_seqs] stay as they were.  Infinite or NaN keys and values
+ * stay with the rows that see them.  q / out are FP32 rows [..][heads * hd] with strides ldq / ldo.
+ * Everything is held in 32 bits or more; results are the same on every call.
+ * The bounds are the host's: max_rows rows in q and out, max_new rows of one request, max_kv positions
+ * of one request.  max_rows is kept to (rows behind it are neither read nor written); max_new and
+ * max_kv choose the kernel and its split, lengths above them are right but slow.
+ * ws_dev: ef_hip_paged_attention_workspace_bytes of the same sizes (may be 0: then ws_dev may be NULL). */
+typedef struct {
+  const int32_t *row_start_dev, *kv_len_dev, *table_dev;
+  size_t table_ld, n_seqs, max_rows, max_new, max_kv;
+} ef_hip_paged_batch;
+size_t ef_hip_paged_attention_workspace_bytes(size_t heads, const ef_hip_page_pool* pool, size_t n_seqs, size_t max_rows,
+                                              size_t max_new, size_t max_kv);
+int ef_hip_paged_attention(const float* q_dev, size_t ldq, float* out_dev, size_t ldo, size_t heads,
+                           const ef_hip_page_pool* pool, const ef_hip_paged_batch* batch, float scale, void* ws_dev,
+                           size_t ws_bytes, void* stream);
+
+/* Causal attention over whole prompts packed one after another, without a cache: rows row_start_dev[r] ..
+ * row_start_dev[r + 1] of q, k and v are prompt r, whose row i sees its rows 0 .. i.  k / v rows hold [KV * hd]
+ * values of `qtype` (F32, F16 or BF16) with strides ldk / ldv in values; the rest as in
+ * ef_hip_paged_attention.  Strides and addresses at multiples of 16 bytes, hd a multiple of 8 up to 256. */
+size_t ef_hip_packed_attention_workspace_bytes(size_t heads, size_t KV, size_t hd, int qtype, size_t n_seqs,
+                                               size_t max_rows);
+int ef_hip_packed_attention(const float* q_dev, size_t ldq, const void* k_dev, size_t ldk, const void* v_dev, size_t ldv,
+                            int qtype, float* out_dev, size_t ldo, size_t heads, size_t KV, size_t hd,
+                            const int32_t* row_start_dev, size_t n_seqs, size_t max_rows, float scale, void* ws_dev,
+                            size_t ws_bytes, void* stream);
+
 /* ---- .efq model files -------------------------------------------------------------------------
  * ef::QuantFile (include/ef/qfile.h:95-124).  ef_hip_efq_open maps a file and validates it as
  * QuantFile::open / parse_efq do (src/qfile.cpp:125-243): magic, version, header length, strict
