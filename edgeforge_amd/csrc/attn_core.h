@@ -1,0 +1,202 @@
+// What the kernels of attention over pages and packed prompts share (paged_attention.hip, attn_few.hip,
+// attn_tiles.hip):
+//   out = sum_j p_j v_j / sum_j p_j,  p_j = 2^(c2 s_j - sub),  s_j = q . k_j,  c2 = scale log2(e),
+// sub the rounded c2 max_j s_j so far (a rescaling is by the difference of two sub, so that it is consistent
+// with the terms already summed however large the scores' common part is).
+#pragma once
+
+#include "paging.h"
+
+#pragma clang fp contract(off)
+
+namespace efh {
+
+typedef float f4v __attribute__((ext_vector_type(4)));
+typedef float f2v __attribute__((ext_vector_type(2)));
+typedef _Float16 h8v __attribute__((ext_vector_type(8)));
+typedef _Float16 h2v __attribute__((ext_vector_type(2)));
+typedef __bf16 b8v __attribute__((ext_vector_type(8)));
+typedef uint32_t u4v __attribute__((ext_vector_type(4)));
+typedef uint32_t u2v __attribute__((ext_vector_type(2)));
+
+struct RowsArgs {
+  const float* q;
+  float* out;
+  long ldq, ldo;
+  int H, KV, hd;
+  const int32_t *row_start, *kv_len;  // kv_len null: packed
+  int n_seqs, max_rows;
+  float c2;
+  KvSource kv;
+};
+
+// 8 values from a 16-byte boundary (32 bytes in FP32) as FP32.
+template <class T>
+__device__ __forceinline__ void load8(const T* p, float (&x)[8]) {
+  if constexpr (sizeof(T) == 4) {
+    const f4v a = *reinterpret_cast<const f4v*>(p), b = *reinterpret_cast<const f4v*>(p + 4);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[i] = a[i];
+      x[4 + i] = b[i];
+    }
+  } else if constexpr (std::is_same_v<T, _Float16>) {
+    const h8v a = *reinterpret_cast<const h8v*>(p);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = static_cast<float>(a[i]);
+  } else {
+    const b8v a = *reinterpret_cast<const b8v*>(p);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = static_cast<float>(a[i]);
+  }
+}
+
+// What the positions [j0, j1) give one (row, head) pair, by a whole wave: a lane takes every 64th position's
+// score and dims lane + 64 u of the output.  q is in LDS.  The sums join (sub, l, o); only seen positions are
+// read, so infinities and NaN elsewhere do not matter.
+template <class T, bool PAGED>
+__device__ void wave_attend(const KvSource& src, int g, int hd, long base, const float* q, float c2, int j0, int j1,
+                            float* sub, double* l, float (&o)[4]) {
+  const int lane = threadIdx.x & (kWave - 1);
+  const T *kp = static_cast<const T*>(src.k), *vp = static_cast<const T*>(src.v);
+  for (int c = j0; c < j1; c += kWave) {
+    const int j = c + lane;
+    long ko = 0, vo = 0;
+    const bool seen = j < j1 && kv_offset<PAGED>(src, g, hd, base, j, &ko, &vo);
+    float s = -INFINITY;
+    if (seen) {
+      float part[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+      for (int d = 0; d < hd; d += 8) {
+        float x[8];
+        load8(kp + ko + d, x);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) part[i] = fmaf(x[i], q[d + i], part[i]);
+      }
+      s = ((part[0] + part[1]) + (part[2] + part[3])) + ((part[4] + part[5]) + (part[6] + part[7]));
+    }
+    const float top = wave_max_dpp(s) * c2;
+    float al = 1.0f;
+    if (top > *sub) {
+      al = *sub == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(*sub - top);
+      *l *= static_cast<double>(al);
+      *sub = top;
+    }
+    const float from = *sub == -INFINITY ? 0.0f : *sub;
+    const float p = seen ? __builtin_amdgcn_exp2f(fmaf(s, c2, -from)) : 0.0f;
+    *l += static_cast<double>(p);
+    float oc[4] = {0, 0, 0, 0};  // the chunk's own sum: no chain of additions is longer than 64 or the chunks
+    for (uint64_t todo = __ballot(seen); todo; todo &= todo - 1) {
+      const int at = __ffsll(static_cast<unsigned long long>(todo)) - 1;
+      const float pj = __shfl(p, at, kWave);
+      const long off = __shfl(vo, at, kWave);
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (lane + 64 * u < hd) oc[u] = fmaf(pj, static_cast<float>(vp[off + lane + 64 * u]), oc[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) o[u] = fmaf(o[u], al, oc[u]);
+  }
+}
+
+// ---- matrix-core operands ------------------------------------------------------------------------------
+// FP32 accuracy from 16-bit products: an FP32 operand is split into 16-bit parts whose sum keeps 22 bits or more, and
+// the parts' products are summed in FP32 by the matrix cores.
+//   FP16 keys and values: 2 parts (11 bits each, both rounded to nearest).  Their small range is met by a power of
+//     two: queries are brought to 2^14 .. 2^15 by one that c2 takes back, and p is formed as 2^14 p (the
+//     offset stays in sub), so that what falls below the smallest half is below 2^-39 of the largest.
+//   BF16: 3 parts (8 bits each, truncated, exact in all 24 bits and FP32's range).
+template <class T>
+struct Parts;
+template <>
+struct Parts<_Float16> {
+  static constexpr int N = 2;
+  static constexpr float kSubOffset = 14.0f;
+  typedef h8v V;
+};
+template <>
+struct Parts<__bf16> {
+  static constexpr int N = 3;
+  static constexpr float kSubOffset = 0.0f;
+  typedef b8v V;
+};
+
+// Two FP32 values' bfloat16 high halves in one word (truncation).
+__device__ __forceinline__ uint32_t high_halves(float lo, float hi) {
+  return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u);
+}
+
+// x[0..7] as parts: word i of part p holds values 2 i and 2 i + 1.
+template <class T>
+__device__ __forceinline__ void split8(const float (&x)[8], u4v (&part)[Parts<T>::N]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float a = x[2 * i], b = x[2 * i + 1];
+    if constexpr (std::is_same_v<T, _Float16>) {
+      const h2v hi = __builtin_convertvector((f2v{a, b}), h2v);
+      part[0][i] = __builtin_bit_cast(uint32_t, hi);
+      const h2v lo = __builtin_convertvector((f2v{a - static_cast<float>(hi[0]), b - static_cast<float>(hi[1])}), h2v);
+      part[1][i] = __builtin_bit_cast(uint32_t, lo);
+    } else {
+      part[0][i] = high_halves(a, b);
+      a -= __uint_as_float(__float_as_uint(a) & 0xFFFF0000u);
+      b -= __uint_as_float(__float_as_uint(b) & 0xFFFF0000u);
+      part[1][i] = high_halves(a, b);
+      a -= __uint_as_float(__float_as_uint(a) & 0xFFFF0000u);
+      b -= __uint_as_float(__float_as_uint(b) & 0xFFFF0000u);
+      part[2][i] = high_halves(a, b);
+    }
+  }
+}
+
+template <class T>
+__device__ __forceinline__ f4v mfma16(u4v a, u4v b, f4v c) {
+  if constexpr (std::is_same_v<T, _Float16>)
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8v, a), __builtin_bit_cast(h8v, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8v, a), __builtin_bit_cast(b8v, b), c, 0, 0, 0);
+}
+
+// Over the lanes that differ in bit 4 and bit 5 (one column of a 16-wide matrix tile).
+__device__ __forceinline__ float column_max(float v) {
+  const u2v a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const u2v b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float column_sum(float v) {
+  const u2v a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  const u2v b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+// The power of two that brings a row of FP16 queries whose largest magnitude is `top` to 2^14 .. 2^15 (1 for a row of
+// zeros, infinities or NaN), as its exponent.
+__device__ __forceinline__ int query_exponent(float top) {
+  const int e = static_cast<int>(__float_as_uint(top) >> 23 & 255);
+  return top == 0.0f || e == 255 ? 0 : min(141 - e, 127);
+}
+
+// ---- the split over positions ----------------------------------------------------------------------------
+// A request's positions are cut into `splits` ranges of `span` (the last one takes the rest, whatever the length);
+// each range's (sub, l) and unnormalised sums go to the workspace, and attention_join_kernel adds them.
+struct SplitArgs {
+  int splits, span;
+  float* part;  // [splits][rows * H][hd]
+  f2v* stat;    // [splits][rows * H]: sub, l
+};
+__host__ __device__ __forceinline__ int splits_of(int kv, int splits, int span) {
+  const int need = kv <= 0 ? 1 : (kv - 1) / span + 1;
+  return need < splits ? need : splits;
+}
+
+struct AttnTask {
+  RowsArgs r;
+  SplitArgs s;
+  int tiles;     // few-rows kernel: workgroups per (request, KV head) along its rows
+  int few_most;  // (row, head) pairs of a KV head up to which a request is the few-rows kernel's
+};
+
+int launch_attention_few(const AttnTask& t, int qtype, hipStream_t s);
+
+}  // namespace efh

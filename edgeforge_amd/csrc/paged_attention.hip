@@ -1,99 +1,14 @@
 // Attention over pages and over packed prompts: requests of different lengths in one call.
-//   out = sum_j p_j v_j / sum_j p_j,  p_j = 2^(c2 s_j - sub),  s_j = q . k_j,  c2 = scale log2(e),
-// sub the rounded c2 max_j s_j so far (a rescaling is by the difference of two sub, so that it is consistent
-// with the terms already summed however large the scores' common part is).
+// Entry points and the choice of kernel.
 #include <algorithm>
 #include <cmath>
 
-#include "paging.h"
+#include "attn_core.h"
 
 #pragma clang fp contract(off)
 
 namespace efh {
 namespace {
-
-typedef float f4v __attribute__((ext_vector_type(4)));
-typedef _Float16 h8v __attribute__((ext_vector_type(8)));
-typedef __bf16 b8v __attribute__((ext_vector_type(8)));
-
-struct RowsArgs {
-  const float* q;
-  float* out;
-  long ldq, ldo;
-  int H, KV, hd;
-  const int32_t *row_start, *kv_len;  // kv_len null: packed
-  int n_seqs, max_rows;
-  float c2;
-  KvSource kv;
-};
-
-// 8 values from a 16-byte boundary (32 bytes in FP32) as FP32.
-template <class T>
-__device__ __forceinline__ void load8(const T* p, float (&x)[8]) {
-  if constexpr (sizeof(T) == 4) {
-    const f4v a = *reinterpret_cast<const f4v*>(p), b = *reinterpret_cast<const f4v*>(p + 4);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      x[i] = a[i];
-      x[4 + i] = b[i];
-    }
-  } else if constexpr (std::is_same_v<T, _Float16>) {
-    const h8v a = *reinterpret_cast<const h8v*>(p);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = static_cast<float>(a[i]);
-  } else {
-    const b8v a = *reinterpret_cast<const b8v*>(p);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = static_cast<float>(a[i]);
-  }
-}
-
-// What the positions [j0, j1) give one (row, head) pair, by a whole wave: a lane takes every 64th position's
-// score and dims lane + 64 u of the output.  q is in LDS.  The sums join (sub, l, o); only seen positions are
-// read, so infinities and NaN elsewhere do not matter.
-template <class T, bool PAGED>
-__device__ void wave_attend(const KvSource& src, int g, int hd, long base, const float* q, float c2, int j0, int j1,
-                            float* sub, double* l, float (&o)[4]) {
-  const int lane = threadIdx.x & (kWave - 1);
-  const T *kp = static_cast<const T*>(src.k), *vp = static_cast<const T*>(src.v);
-  for (int c = j0; c < j1; c += kWave) {
-    const int j = c + lane;
-    long ko = 0, vo = 0;
-    const bool seen = j < j1 && kv_offset<PAGED>(src, g, hd, base, j, &ko, &vo);
-    float s = -INFINITY;
-    if (seen) {
-      float part[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-      for (int d = 0; d < hd; d += 8) {
-        float x[8];
-        load8(kp + ko + d, x);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) part[i] = fmaf(x[i], q[d + i], part[i]);
-      }
-      s = ((part[0] + part[1]) + (part[2] + part[3])) + ((part[4] + part[5]) + (part[6] + part[7]));
-    }
-    const float top = wave_max_dpp(s) * c2;
-    float al = 1.0f;
-    if (top > *sub) {
-      al = *sub == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(*sub - top);
-      *l *= static_cast<double>(al);
-      *sub = top;
-    }
-    const float from = *sub == -INFINITY ? 0.0f : *sub;
-    const float p = seen ? __builtin_amdgcn_exp2f(fmaf(s, c2, -from)) : 0.0f;
-    *l += static_cast<double>(p);
-    float oc[4] = {0, 0, 0, 0};  // the chunk's own sum: no chain of additions is longer than 64 or the chunks
-    for (uint64_t todo = __ballot(seen); todo; todo &= todo - 1) {
-      const int at = __ffsll(static_cast<unsigned long long>(todo)) - 1;
-      const float pj = __shfl(p, at, kWave);
-      const long off = __shfl(vo, at, kWave);
-#pragma unroll
-      for (int u = 0; u < 4; ++u)
-        if (lane + 64 * u < hd) oc[u] = fmaf(pj, static_cast<float>(vp[off + lane + 64 * u]), oc[u]);
-    }
-#pragma unroll
-    for (int u = 0; u < 4; ++u) o[u] = fmaf(o[u], al, oc[u]);
-  }
-}
 
 // One wave per (row, query head).
 constexpr int kRowWaves = 4;
@@ -153,6 +68,31 @@ int launch_rows(const RowsArgs& a, int qtype, hipStream_t s) {
   return EF_HIP_OK;
 }
 
+// How a call of paged attention runs.
+struct PagedPlan {
+  bool few = false;
+  int tiles = 1, splits = 1, span = 128;
+  size_t bytes = 0;  // workspace
+};
+constexpr int kFewPairs = 16, kSpanStep = 128, kSpanLeast = 256, kSpanMost = 4096, kSplitWorkgroups = 1024;
+
+PagedPlan plan_paged(size_t H, size_t KV, size_t hd, size_t n_seqs, size_t max_rows, size_t max_new, size_t max_kv) {
+  PagedPlan p;
+  const size_t pairs = std::max<size_t>(max_new, 1) * (H / KV);
+  p.few = pairs <= 64;
+  if (!p.few) return p;
+  p.tiles = static_cast<int>((pairs + kFewPairs - 1) / kFewPairs);
+  const size_t wgs = n_seqs * KV * p.tiles, want = (kSplitWorkgroups + wgs - 1) / wgs;
+  const size_t longest = std::max<size_t>(max_kv, 1);
+  size_t span = std::min<size_t>(std::max<size_t>((longest + want - 1) / want, kSpanLeast), kSpanMost);
+  span = std::max(span, (longest + 1023) / 1024);
+  span = (span + kSpanStep - 1) / kSpanStep * kSpanStep;
+  p.span = static_cast<int>(span);
+  p.splits = static_cast<int>((longest + span - 1) / span);
+  if (p.splits > 1) p.bytes = max_rows * H * p.splits * (hd + 2) * sizeof(float);
+  return p;
+}
+
 }  // namespace
 }  // namespace efh
 
@@ -162,8 +102,10 @@ extern "C" {
 
 size_t ef_hip_paged_attention_workspace_bytes(size_t heads, const ef_hip_page_pool* pool, size_t n_seqs, size_t max_rows,
                                               size_t max_new, size_t max_kv) {
-  (void)heads, (void)pool, (void)n_seqs, (void)max_rows, (void)max_new, (void)max_kv;
-  return 0;
+  if (check_page_pool(pool, "paged_attention") != EF_HIP_OK || heads < 1 || heads > 65535 || heads % pool->KV != 0 ||
+      n_seqs < 1 || max_rows > (size_t(1) << 30) || max_kv > 0x7FFFFFFF)
+    return 0;
+  return plan_paged(heads, pool->KV, pool->hd, n_seqs, max_rows, max_new, max_kv).bytes;
 }
 
 int ef_hip_paged_attention(const float* q, size_t ldq, float* out, size_t ldo, size_t heads, const ef_hip_page_pool* pool,
@@ -190,10 +132,23 @@ int ef_hip_paged_attention(const float* q, size_t ldq, float* out, size_t ldo, s
   a.c2 = scale * 1.44269504088896340736f;
   a.kv = KvSource{pool->k_dev, pool->v_dev, 0, 0, b.table_dev, static_cast<long>(b.table_ld),
                   static_cast<long>(pool_stride(*pool)), log2_of(pool->page_size), static_cast<int>(pool->n_pages)};
-  (void)ws, (void)ws_bytes;
+  EFH_CHECK(b.max_kv <= 0x7FFFFFFF, "paged_attention: max_kv too large");
+  const PagedPlan p = plan_paged(heads, pool->KV, pool->hd, b.n_seqs, b.max_rows, b.max_new, b.max_kv);
+  EFH_CHECK(p.bytes == 0 || (ws != nullptr && ws_bytes >= p.bytes && aligned16(ws)),
+            "paged_attention: the workspace must have ef_hip_paged_attention_workspace_bytes bytes, at a multiple of 16");
+  EFH_CHECK(b.n_seqs * pool->KV <= size_t(0x7FFFFFFF) / p.tiles, "paged_attention: too many requests and heads");
   EFH_RC(require_ready());
   if (b.max_rows == 0) return EF_HIP_OK;
-  return launch_rows<true>(a, pool->qtype, pick(stream));
+  if (!p.few) return launch_rows<true>(a, pool->qtype, pick(stream));
+  AttnTask t{};
+  t.r = a;
+  t.tiles = p.tiles;
+  t.few_most = 0x7FFFFFFF;
+  t.s.splits = p.splits;
+  t.s.span = p.span;
+  t.s.part = static_cast<float*>(ws);
+  t.s.stat = reinterpret_cast<f2v*>(t.s.part + b.max_rows * heads * p.splits * pool->hd);
+  return launch_attention_few(t, pool->qtype, pick(stream));
 }
 
 size_t ef_hip_packed_attention_workspace_bytes(size_t heads, size_t KV, size_t hd, int qtype, size_t n_seqs,
