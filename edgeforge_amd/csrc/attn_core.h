@@ -102,15 +102,23 @@ __device__ void wave_attend(const KvSource& src, int g, int hd, long base, const
 // FP32 accuracy from 16-bit products: an FP32 operand is split into 16-bit parts whose sum keeps 22 bits or more, and
 // the parts' products are summed in FP32 by the matrix cores.
 //   FP16 keys and values: 2 parts (11 bits each, both rounded to nearest).  Their small range is met by a power of
-//     two: queries are brought to 2^14 .. 2^15 by one that c2 takes back, and p is formed as 2^14 p (the
-//     offset stays in sub), so that what falls below the smallest half is below 2^-39 of the largest.
+//     two: queries are brought to 2^14 .. 2^15 by one that c2 takes back, and p is formed as 2^7 p (the
+//     offset stays in sub), so that what falls below the smallest half is below 2^-31 of the largest.
 //   BF16: 3 parts (8 bits each, truncated, exact in all 24 bits and FP32's range).
+// FP32 pages are split into 3 BF16 parts too where the matrix tiles are large (6 products; what is dropped is below
+// 2^-21 of a product, at random signs).
 template <class T>
 struct Parts;
 template <>
+struct Parts<float> {
+  static constexpr int N = 3;
+  static constexpr float kSubOffset = 0.0f;
+  typedef b8v V;
+};
+template <>
 struct Parts<_Float16> {
   static constexpr int N = 2;
-  static constexpr float kSubOffset = 14.0f;
+  static constexpr float kSubOffset = 7.0f;
   typedef h8v V;
 };
 template <>
@@ -177,26 +185,36 @@ __device__ __forceinline__ int query_exponent(float top) {
   return top == 0.0f || e == 255 ? 0 : min(141 - e, 127);
 }
 
+// A running sub is raised only when a score passes it by this much (in powers of two; the weights then reach 2^8, and
+// 2^15 with the offset of FP16): with one pass over many positions a new maximum comes often, a much larger one
+// hardly ever.
+constexpr float kSubSlack = 8.0f;
+
 // ---- the split over positions ----------------------------------------------------------------------------
 // A request's positions are cut into `splits` ranges of `span` (the last one takes the rest, whatever the length);
 // each range's (sub, l) and unnormalised sums go to the workspace, and attention_join_kernel adds them.
-struct SplitArgs {
+struct Split {
   int splits, span;
-  float* part;  // [splits][rows * H][hd]
-  f2v* stat;    // [splits][rows * H]: sub, l
 };
-__host__ __device__ __forceinline__ int splits_of(int kv, int splits, int span) {
-  const int need = kv <= 0 ? 1 : (kv - 1) / span + 1;
-  return need < splits ? need : splits;
+__host__ __device__ __forceinline__ int splits_of(int kv, Split s) {
+  const int need = kv <= 0 ? 1 : (kv - 1) / s.span + 1;
+  return need < s.splits ? need : s.splits;
 }
 
 struct AttnTask {
   RowsArgs r;
-  SplitArgs s;
+  Split few_split, tile_split;
+  float* part;  // [splits][rows * H][hd]
+  f2v* stat;    // [splits][rows * H]: sub, l
   int tiles;     // few-rows kernel: workgroups per (request, KV head) along its rows
-  int few_most;  // (row, head) pairs of a KV head up to which a request is the few-rows kernel's
+  int few_most;  // (row, head) pairs of a KV head up to which a request is the few-rows kernel's, not the tiles kernel's
 };
 
+// (row, head) pairs of a KV head in a workgroup of the tiles kernel
+constexpr int kTilePairs = 128;
+
+int launch_attention_tiles(const AttnTask& t, int qtype, bool paged, hipStream_t s);
+int launch_attention_join(const AttnTask& t, hipStream_t s);
 int launch_attention_few(const AttnTask& t, int qtype, hipStream_t s);
 
 }  // namespace efh

@@ -28,6 +28,7 @@ __global__ __launch_bounds__(kFewWaves * kWave, HDP == 256 ? 1 : (HDP == 64 ? 3 
   constexpr int KT = F32 ? 16 : 32, TILES = KT / 16, DP = HDP / 16;
   constexpr int KW = F32 ? HDP / 16 : HDP / 32;  // 16-byte pieces of a key row in a lane
   constexpr int VROWS = 4 * TILES, VW = F32 ? DP / 4 : DP * 2 / 16 + (DP == 4);  // value rows of a lane, 16-byte pieces each (8 bytes for 4 halves)
+  constexpr float OFFSET = F32 ? 0.0f : Parts<T>::kSubOffset;
   constexpr int PAIRS = 16 * NT, LDO = HDP + 4;
   __shared__ float o_s[kFewWaves][PAIRS * LDO];
   __shared__ f2v stat_s[kFewWaves][PAIRS];
@@ -46,9 +47,9 @@ __global__ __launch_bounds__(kFewWaves * kWave, HDP == 256 ? 1 : (HDP == 64 ? 3 
   const int kv_len = a.kv_len[req];
   const int kv = static_cast<int>(min(static_cast<long>(kv_len), a.kv.table_ld << a.kv.page_shift));
   if (n <= 0 || static_cast<long>(n) * G > t.few_most) return;
-  const int ns = splits_of(kv, t.s.splits, t.s.span);
+  const int ns = splits_of(kv, t.few_split);
   if (split >= ns) return;
-  const int j0 = split * t.s.span, j1 = split == t.s.splits - 1 ? max(kv, 0) : min(max(kv, 0), j0 + t.s.span);
+  const int j0 = split * t.few_split.span, j1 = split == t.few_split.splits - 1 ? max(kv, 0) : min(max(kv, 0), j0 + t.few_split.span);
   const int before = kv_len - n;  // row i sees positions 0 .. before + i
   const int sh = a.kv.page_shift, pmask = (1 << sh) - 1;
   const T *kp = static_cast<const T*>(a.kv.k), *vp = static_cast<const T*>(a.kv.v);
@@ -62,7 +63,7 @@ __global__ __launch_bounds__(kFewWaves * kWave, HDP == 256 ? 1 : (HDP == 64 ? 3 
 
   for (int tile = tile0; tile * PAIRS < n * G; tile += t.tiles) {
     // ---- queries -------------------------------------------------------------------------------------
-    constexpr int NS = F32 ? 1 : Parts<std::conditional_t<F32, _Float16, T>>::N;
+    constexpr int NS = F32 ? 1 : Parts<T>::N;
     f4v qf[F32 ? NT : 1][KW];
     u4v qp[F32 ? 1 : NT][KW][NS];
     float c2[NT];
@@ -101,7 +102,7 @@ __global__ __launch_bounds__(kFewWaves * kWave, HDP == 256 ? 1 : (HDP == 64 ? 3 
             for (int u = 0; u < 8; ++u) x[i][u] = ldexpf(x[i][u], e);
         }
 #pragma unroll
-        for (int i = 0; i < KW; ++i) split8<std::conditional_t<F32, _Float16, T>>(x[i], qp[nt][i]);
+        for (int i = 0; i < KW; ++i) split8<T>(x[i], qp[nt][i]);
       }
     }
     const int all_see = min(before + tile * PAIRS / G + 1, kv);  // positions that every row of the tile sees
@@ -182,13 +183,13 @@ __global__ __launch_bounds__(kFewWaves * kWave, HDP == 256 ? 1 : (HDP == 64 ? 3 
     };
 
     f4v o[NT][DP];
-    float mx[NT], sub[NT], l[NT];
+    float sub[NT], l[NT];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
       for (int d = 0; d < DP; ++d) o[nt][d] = f4v{0, 0, 0, 0};
-      mx[nt] = -INFINITY;
-      sub[nt] = l[nt] = 0.0f;
+      sub[nt] = -INFINITY;
+      l[nt] = 0.0f;
     }
     constexpr int STEP = kFewWaves * KT;
     int c = j0 + wave * KT;
@@ -259,22 +260,22 @@ __global__ __launch_bounds__(kFewWaves * kWave, HDP == 256 ? 1 : (HDP == 64 ? 3 
 #pragma unroll
           for (int r = 0; r < 4; ++r) cm = fmaxf(cm, sc[nt][u][r]);
         cm = column_max(cm);
-        if (__any(cm > mx[nt])) {
-          const float nm = fmaxf(mx[nt], cm);
-          const float ns_ = nm == -INFINITY ? 0.0f : nm * c2[nt] - (F32 ? 0.0f : Parts<std::conditional_t<F32, _Float16, T>>::kSubOffset);
-          const float al = mx[nt] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(sub[nt] - ns_);
-          mx[nt] = nm;
-          sub[nt] = ns_;
+        const float high = cm * c2[nt] - OFFSET;
+        if (__any(high > sub[nt] + kSubSlack)) {
+          const float to = fmaxf(sub[nt], high);
+          const float al = to == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(sub[nt] - to);
+          sub[nt] = to;
           l[nt] *= al;
 #pragma unroll
           for (int d = 0; d < DP; ++d) o[nt][d] *= al;
         }
+        const float from = sub[nt] == -INFINITY ? 0.0f : sub[nt];
         float sum = 0.0f;
 #pragma unroll
         for (int u = 0; u < TILES; ++u)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            p[nt][4 * u + r] = __builtin_amdgcn_exp2f(fmaf(sc[nt][u][r], c2[nt], -sub[nt]));
+            p[nt][4 * u + r] = __builtin_amdgcn_exp2f(fmaf(sc[nt][u][r], c2[nt], -from));
             sum += p[nt][4 * u + r];
           }
         l[nt] += sum;
@@ -290,7 +291,7 @@ __global__ __launch_bounds__(kFewWaves * kWave, HDP == 256 ? 1 : (HDP == 64 ? 3 
       } else {
         u4v pp[NT][NS];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) split8<std::conditional_t<F32, _Float16, T>>(p[nt], pp[nt]);
+        for (int nt = 0; nt < NT; ++nt) split8<T>(p[nt], pp[nt]);
 #pragma unroll
         for (int d = 0; d < DP; ++d) {
           u4v v;  // dim m DP + d of the lane's eight value rows
@@ -314,7 +315,7 @@ __global__ __launch_bounds__(kFewWaves * kWave, HDP == 256 ? 1 : (HDP == 64 ? 3 
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const float lw = column_sum(l[nt]);
-      if (g4 == 0) stat_s[wave][16 * nt + m] = f2v{mx[nt] == -INFINITY ? -INFINITY : sub[nt], lw};
+      if (g4 == 0) stat_s[wave][16 * nt + m] = f2v{sub[nt], lw};
 #pragma unroll
       for (int r = 0; r < 4; ++r)
 #pragma unroll
@@ -352,8 +353,8 @@ __global__ __launch_bounds__(kFewWaves * kWave, HDP == 256 ? 1 : (HDP == 64 ? 3 
         const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
         *reinterpret_cast<f4v*>(a.out + out_row + d) = acc * inv;
       } else {
-        *reinterpret_cast<f4v*>(t.s.part + part_row * hd + d) = acc;
-        if (d == 0) t.s.stat[part_row] = f2v{top, sum};
+        *reinterpret_cast<f4v*>(t.part + part_row * hd + d) = acc;
+        if (d == 0) t.stat[part_row] = f2v{top, sum};
       }
     }
     if (__syncthreads_or(bad)) {
@@ -377,9 +378,9 @@ __global__ __launch_bounds__(kFewWaves * kWave, HDP == 256 ? 1 : (HDP == 64 ? 3 
           const int d = lane + 64 * u;
           if (d >= hd) continue;
           if (direct) a.out[out_row + d] = ov[u] * inv;
-          else t.s.part[part_row * hd + d] = ov[u];
+          else t.part[part_row * hd + d] = ov[u];
         }
-        if (!direct && lane == 0) t.s.stat[part_row] = f2v{sb, static_cast<float>(ll)};
+        if (!direct && lane == 0) t.stat[part_row] = f2v{sb, static_cast<float>(ll)};
         __builtin_amdgcn_wave_barrier();
       }
     }
@@ -395,18 +396,19 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttnTask t) {
   if (row >= min(a.row_start[a.n_seqs], a.max_rows) || h >= a.H) return;
   const int req = request_of(a.row_start, a.n_seqs, row);
   const int kv = static_cast<int>(min(static_cast<long>(a.kv_len[req]), a.kv.table_ld << a.kv.page_shift));
-  const int ns = splits_of(kv, t.s.splits, t.s.span);
+  const long pairs = static_cast<long>(a.row_start[req + 1] - a.row_start[req]) * (a.H / a.KV);
+  const int ns = splits_of(kv, pairs <= t.few_most ? t.few_split : t.tile_split);
   if (ns == 1) return;
   const long step = static_cast<long>(a.max_rows) * a.H, at = static_cast<long>(row) * a.H + h;
   float top = -INFINITY;
-  for (int s = lane; s < ns; s += kWave) top = fmaxf(top, t.s.stat[s * step + at][0]);
+  for (int s = lane; s < ns; s += kWave) top = fmaxf(top, t.stat[s * step + at][0]);
   top = wave_max_dpp(top);
   float l = 0.0f, o[4] = {0, 0, 0, 0};
   for (int s = 0; s < ns; ++s) {
-    const f2v st = t.s.stat[s * step + at];
+    const f2v st = t.stat[s * step + at];
     const float f = st[0] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(st[0] - top);
     l = fmaf(st[1], f, l);
-    const float* p = t.s.part + (s * step + at) * a.hd;
+    const float* p = t.part + (s * step + at) * a.hd;
 #pragma unroll
     for (int u = 0; u < 4; ++u)
       if (lane + 64 * u < a.hd) o[u] = fmaf(p[lane + 64 * u], f, o[u]);
@@ -420,7 +422,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttnTask t) {
 
 template <class T, int HDP, int NT>
 void run_few(const AttnTask& t, hipStream_t s) {
-  const dim3 grid(t.r.n_seqs * t.r.KV * t.tiles, t.s.splits);
+  const dim3 grid(t.r.n_seqs * t.r.KV * t.tiles, t.few_split.splits);
   if (t.r.kv.page_shift >= 4) attention_few_kernel<T, HDP, NT, true><<<grid, kFewWaves * kWave, 0, s>>>(t);
   else attention_few_kernel<T, HDP, NT, false><<<grid, kFewWaves * kWave, 0, s>>>(t);
 }
@@ -439,10 +441,12 @@ int launch_attention_few(const AttnTask& t, int qtype, hipStream_t s) {
   else if (qtype == EF_QTYPE_F16) run_few_of<_Float16>(t, s);
   else run_few_of<__bf16>(t, s);
   EFH_HIP(hipGetLastError());
-  if (t.s.splits > 1) {
-    attention_join_kernel<<<dim3(t.r.max_rows, (t.r.H + 3) / 4), 256, 0, s>>>(t);
-    EFH_HIP(hipGetLastError());
-  }
+  return EF_HIP_OK;
+}
+
+int launch_attention_join(const AttnTask& t, hipStream_t s) {
+  attention_join_kernel<<<dim3(t.r.max_rows, (t.r.H + 3) / 4), 256, 0, s>>>(t);
+  EFH_HIP(hipGetLastError());
   return EF_HIP_OK;
 }
 

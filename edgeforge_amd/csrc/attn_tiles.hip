@@ -1,0 +1,380 @@
+// Attention of many new rows: chunks over pages, and packed prompts.
+//
+// A workgroup takes 128 (row, query head) pairs of one request and KV head, 32 to a wave, and walks the positions
+// they see in tiles of BN: a tile's keys and values are staged in LDS once for all pairs, loaded into registers
+// while the tile before is used.  S^T = K Q^T by v_mfma_f32_32x32x16 puts a pair's scores in its own two lanes (D:
+// positions 8 (i / 4) + 4 h + i % 4, pair lane % 32, h = lane / 32).  The k slots of a product may hold
+// positions in any order, so the weights feed O^T += V^T P^T from the registers they were computed in, against
+// V read transposed from LDS (ds_read_b64_tr_b16: 16 lanes read four positions' rows of 16 dims and get four
+// positions of a dim each).  16-bit parts of the queries and the weights keep FP32's accuracy (attn_core.h); FP32
+// keys and values are split into three parts as they are staged.
+//
+// Masked positions: scores -inf; rows past the last position or without a page are staged as zeros.  Pairs whose
+// sums come out infinite or NaN are computed again by wave_attend, which reads only what each row sees.
+#include <algorithm>
+
+#include "attn_core.h"
+
+namespace efh {
+namespace {
+
+typedef float f16v __attribute__((ext_vector_type(16)));
+typedef short s4v __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s4v* lds_s4v;
+
+constexpr int kTileWaves = 4, kTileThreads = kTileWaves * kWave;
+
+template <class T>
+__device__ __forceinline__ f16v mfma32(u4v a, u4v b, f16v c) {
+  if constexpr (std::is_same_v<T, _Float16>)
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8v, a), __builtin_bit_cast(h8v, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8v, a), __builtin_bit_cast(b8v, b), c, 0, 0, 0);
+}
+
+__device__ __forceinline__ float half_max(float v) {  // over lanes l and l + 32
+  const u2v b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float half_sum(float v) {
+  const u2v b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+// Request r's tiles have the places floor(start[r] G / 128) + r on: at least as many as it needs, without a sum over
+// the requests before it.  The request of place x, by a whole wave.
+__device__ __forceinline__ long tile_place(const RowsArgs& a, int r) {
+  return static_cast<long>(a.row_start[r]) * (a.H / a.KV) / kTilePairs + r;
+}
+__device__ __forceinline__ int request_of_place(const RowsArgs& a, long x) {
+  const int lane = threadIdx.x & (kWave - 1);
+  int lo = 0, len = a.n_seqs;
+  while (len > 1) {
+    const int step = (len + kWave - 1) / kWave, i = lane * step;
+    const uint64_t below = __ballot(i < len && tile_place(a, lo + i) <= x);
+    const int last = max(__popcll(below) - 1, 0) * step;
+    lo += last;
+    len = min(step, len - last);
+  }
+  return __builtin_amdgcn_readfirstlane(lo);
+}
+
+template <class T, int HDP, bool PAGED>
+struct TileShape {
+  static constexpr bool F32 = sizeof(T) == 4;
+  static constexpr int BN = HDP == 256 || (F32 && HDP >= 128) ? 32 : 64;  // positions of a tile
+  static constexpr int PLANES = F32 ? 3 : 1;                    // 16-bit planes of a key or value
+  static constexpr int LDK = HDP + 8, LDV = HDP + 16;           // 16-bit values between rows: no bank conflicts
+  static constexpr int UNITS = BN * HDP / 8 / kTileThreads;     // groups of 8 values that a thread stages
+};
+
+template <class T, int HDP, bool PAGED>
+__global__ __launch_bounds__(kTileThreads, HDP == 64 && sizeof(T) == 2 ? 3 : HDP <= 128 ? 2 : 1) void attention_tiles_kernel(AttnTask t) {
+  using Sh = TileShape<T, HDP, PAGED>;
+  constexpr bool F32 = Sh::F32;
+  constexpr int BN = Sh::BN, SUB = BN / 32, PLANES = Sh::PLANES, LDK = Sh::LDK, LDV = Sh::LDV, UNITS = Sh::UNITS;
+  constexpr int KK = HDP / 16, DT = HDP / 32, NS = Parts<T>::N;
+  constexpr float OFFSET = Parts<T>::kSubOffset;
+  __shared__ __attribute__((aligned(16))) uint16_t ks[PLANES * BN * LDK];
+  __shared__ __attribute__((aligned(16))) uint16_t vs[PLANES * BN * LDV];
+  __shared__ uint32_t ok_s[BN / 4];  // a byte per position: whether a page holds it
+  __shared__ int lost_s;             // some tile so far had a position without a page
+
+  const RowsArgs& a = t.r;
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid & (kWave - 1);
+  const int col = lane & 31, h = lane >> 5;
+  const int G = a.H / a.KV, hd = a.hd;
+  // the last places first: a request's last rows see the most positions
+  const int kvh = blockIdx.x % a.KV;
+  const long place = static_cast<long>(gridDim.x / a.KV) - 1 - blockIdx.x / a.KV;
+  const int req = request_of_place(a, place);
+  const int first = a.row_start[req], n = min(a.row_start[req + 1], a.max_rows) - first;
+  const long tile = place - tile_place(a, req);
+  if (n <= 0 || tile * kTilePairs >= static_cast<long>(n) * G || static_cast<long>(n) * G <= t.few_most) return;
+  int before, kv;
+  long base;
+  if constexpr (PAGED) {
+    const int kv_len = a.kv_len[req];
+    kv = static_cast<int>(min(static_cast<long>(kv_len), a.kv.table_ld << a.kv.page_shift));
+    before = kv_len - n;
+    base = req * a.kv.table_ld;
+  } else {
+    kv = n;
+    before = 0;
+    base = first;
+  }
+  const int ns = splits_of(kv, t.tile_split), split = blockIdx.y;
+  if (split >= ns) return;
+
+  // ---- this lane's pair --------------------------------------------------------------------------------
+  const int pairs = n * G;  // above few_most, and below 2^31 (checked on the host)
+  const int pair0 = static_cast<int>(tile) * kTilePairs, pair = pair0 + 32 * wave + col;
+  const bool active = pair < pairs;
+  const int row = active ? pair / G : 0, head = kvh * G + (active ? pair - row * G : 0);
+  const int seen = active ? min(before + row + 1, kv) : 0;
+  const int tile_last = min(pair0 + kTilePairs, pairs) - 1;
+  // positions: those of the split that the tile's last row sees
+  const int j0 = split * t.tile_split.span;
+  const int j1 = min(split == t.tile_split.splits - 1 ? kv : min(kv, j0 + t.tile_split.span), min(before + tile_last / G + 1, kv));
+  const bool busy = pair0 + 32 * wave < pairs;  // a wave without a pair only stages
+  const int all_see = min(before + (pair0 + 32 * wave) / G + 1, kv);  // positions that every row of the wave sees
+
+  u4v qp[KK][NS];
+  float c2 = a.c2;
+  {
+    const float* q = a.q + static_cast<long>(first + row) * a.ldq + static_cast<long>(head) * hd;
+    float top = 0.0f;
+    int e = 0;
+    if constexpr (std::is_same_v<T, _Float16>) {
+#pragma unroll
+      for (int k = 0; k < KK; ++k) {
+        float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+        if (16 * k + 8 * h < hd) load8(q + 16 * k + 8 * h, x);
+#pragma unroll
+        for (int u = 0; u < 8; ++u) top = fmaxf(top, fabsf(x[u]));
+      }
+      e = query_exponent(half_max(top));
+      c2 = ldexpf(c2, -e);
+    }
+#pragma unroll
+    for (int k = 0; k < KK; ++k) {
+      float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+      if (16 * k + 8 * h < hd) load8(q + 16 * k + 8 * h, x);
+      if constexpr (std::is_same_v<T, _Float16>) {
+#pragma unroll
+        for (int u = 0; u < 8; ++u) x[u] = ldexpf(x[u], e);
+      }
+      split8<T>(x, qp[k]);
+    }
+  }
+
+  // ---- staging -------------------------------------------------------------------------------------------
+  constexpr int ROW_UNITS = HDP / 8, WORDS = F32 ? 2 : 1;
+  u4v kr[UNITS][WORDS], vr[UNITS][WORDS];
+  bool real[UNITS];
+  const int unit_col = 8 * (tid % ROW_UNITS), unit_row = tid / ROW_UNITS;  // unit u: row unit_row + u * 256 / ROW_UNITS
+  const bool in_row = unit_col < hd;
+  const T *kp = static_cast<const T*>(a.kv.k), *vp = static_cast<const T*>(a.kv.v);
+  auto fetch = [&](int c) {
+#pragma unroll
+    for (int u = 0; u < UNITS; ++u) {
+      const int j = c + unit_row + u * (kTileThreads / ROW_UNITS);
+      long ko = 0, vo = 0;
+      real[u] = j < j1 && kv_offset<PAGED>(a.kv, kvh, hd, base, j, &ko, &vo);
+#pragma unroll
+      for (int w = 0; w < WORDS; ++w) kr[u][w] = vr[u][w] = u4v{0, 0, 0, 0};
+      if (real[u] && in_row) {
+#pragma unroll
+        for (int w = 0; w < WORDS; ++w) {
+          kr[u][w] = *reinterpret_cast<const u4v*>(kp + ko + unit_col + 4 * w);
+          vr[u][w] = *reinterpret_cast<const u4v*>(vp + vo + unit_col + 4 * w);
+        }
+      }
+    }
+  };
+  auto put = [&](uint16_t* dst, int ld, const u4v (&x)[WORDS], int r) {
+    if constexpr (F32) {
+      float f[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(x[i / 4][i % 4]);
+      u4v part[3];
+      split8<float>(f, part);
+#pragma unroll
+      for (int p = 0; p < 3; ++p) *reinterpret_cast<u4v*>(dst + (p * BN + r) * ld + unit_col) = part[p];
+    } else {
+      *reinterpret_cast<u4v*>(dst + r * ld + unit_col) = x[0];
+    }
+  };
+  if (tid == 0) lost_s = 0;
+
+  f16v o[DT];
+#pragma unroll
+  for (int d = 0; d < DT; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
+  float sub = -INFINITY, l = 0.0f;
+  if (j0 < j1) fetch(j0);
+  for (int c = j0; c < j1; c += BN) {
+    __syncthreads();  // the tile before is used
+#pragma unroll
+    for (int u = 0; u < UNITS; ++u) {
+      const int r = unit_row + u * (kTileThreads / ROW_UNITS);
+      put(ks, LDK, kr[u], r);
+      put(vs, LDV, vr[u], r);
+      if constexpr (PAGED) {
+        if (unit_col == 0) {
+          reinterpret_cast<uint8_t*>(ok_s)[r] = real[u];
+          if (!real[u] && c + r < j1) lost_s = 1;
+        }
+      }
+    }
+    __syncthreads();
+    if (c + BN < j1) fetch(c + BN);
+    if (!busy) continue;
+
+    f16v sc[SUB];
+#pragma unroll
+    for (int s = 0; s < SUB; ++s) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) sc[s][i] = 0.0f;
+#pragma unroll
+      for (int k = 0; k < KK; ++k) {
+        u4v kf[PLANES];
+#pragma unroll
+        for (int p = 0; p < PLANES; ++p)
+          kf[p] = *reinterpret_cast<const u4v*>(ks + (p * BN + 32 * s + col) * LDK + 16 * k + 8 * h);
+#pragma unroll
+        for (int sum = NS - 1; sum >= 0; --sum)  // the small products first
+#pragma unroll
+          for (int p = 0; p < PLANES; ++p)
+            if (sum - p >= 0) sc[s] = mfma32<T>(kf[p], qp[k][sum - p], sc[s]);
+      }
+    }
+    if (c + BN > all_see) {
+#pragma unroll
+      for (int s = 0; s < SUB; ++s)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (c + 32 * s + 8 * (i / 4) + 4 * h + i % 4 >= seen) sc[s][i] = -INFINITY;
+    }
+    if constexpr (PAGED) {
+      if (lost_s) {
+#pragma unroll
+        for (int s = 0; s < SUB; ++s)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const uint32_t w = ok_s[8 * s + 2 * q + h];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (!(w >> (8 * i) & 255)) sc[s][4 * q + i] = -INFINITY;
+          }
+      }
+    }
+    float cm = -INFINITY;
+#pragma unroll
+    for (int s = 0; s < SUB; ++s)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) cm = fmaxf(cm, sc[s][i]);
+    const float high = half_max(cm) * c2 - OFFSET;
+    if (__any(high > sub + kSubSlack)) {
+      const float to = fmaxf(sub, high);
+      const float al = to == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(sub - to);
+      sub = to;
+      l *= al;
+#pragma unroll
+      for (int d = 0; d < DT; ++d) o[d] *= al;
+    }
+    const float from = sub == -INFINITY ? 0.0f : sub;
+    float sum = 0.0f;
+#pragma unroll
+    for (int s = 0; s < SUB; ++s) {
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {  // 16 positions: one step of the products
+        float p[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          p[i] = __builtin_amdgcn_exp2f(fmaf(sc[s][8 * half + i], c2, -from));
+          sum += p[i];
+        }
+        u4v pp[NS];
+        split8<T>(p, pp);
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+          u4v vf[PLANES];
+#pragma unroll
+          for (int pl = 0; pl < PLANES; ++pl) {
+            uint16_t* at = vs + (pl * BN + 32 * s + 16 * half + 4 * h + (lane & 15) / 4) * LDV + 32 * d + 16 * (lane >> 4 & 1) + 4 * (lane & 3);
+            const s4v lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4v)at);
+            const s4v hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4v)(at + 8 * LDV));
+            const u2v lw = __builtin_bit_cast(u2v, lo), hw = __builtin_bit_cast(u2v, hi);
+            vf[pl] = u4v{lw[0], lw[1], hw[0], hw[1]};
+          }
+#pragma unroll
+          for (int ps = NS - 1; ps >= 0; --ps)
+#pragma unroll
+            for (int pl = 0; pl < PLANES; ++pl)
+              if (ps - pl >= 0) o[d] = mfma32<T>(vf[pl], pp[ps - pl], o[d]);
+        }
+      }
+    }
+    l += sum;
+  }
+
+  // ---- results ---------------------------------------------------------------------------------------------
+  l = half_sum(l);
+  bool bad = !(fabsf(l) < INFINITY);
+#pragma unroll
+  for (int d = 0; d < DT; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) bad = bad || !(fabsf(o[d][i]) < INFINITY);
+  const bool direct = ns == 1;
+  const long out_row = static_cast<long>(first + row) * a.ldo + static_cast<long>(head) * hd;
+  const long part_row = (static_cast<long>(split) * a.max_rows + first + row) * a.H + head;
+  if (active) {
+    const float inv = direct ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f;
+    float* dst = direct ? a.out + out_row : t.part + part_row * hd;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int dim = 32 * d + 8 * q + 4 * h;
+        if (dim < hd) *reinterpret_cast<f4v*>(dst + dim) = f4v{o[d][4 * q], o[d][4 * q + 1], o[d][4 * q + 2], o[d][4 * q + 3]} * inv;
+      }
+    if (!direct && h == 0) t.stat[part_row] = f2v{sub, l};
+  }
+  uint64_t todo = __ballot(bad && active);
+  todo = (todo | todo >> 32) & 0xFFFFFFFFull;
+  __syncthreads();  // the last tile is used
+  float* qs = reinterpret_cast<float*>(ks) + wave * HDP;
+  for (; todo; todo &= todo - 1) {
+    const int who = __ffsll(static_cast<unsigned long long>(todo)) - 1;
+    const int rr = __shfl(row, who, kWave), hh = __shfl(head, who, kWave), lim = min(j1, __shfl(seen, who, kWave));
+    const float* q = a.q + static_cast<long>(first + rr) * a.ldq + static_cast<long>(hh) * hd;
+    for (int d = lane; d < hd; d += kWave) qs[d] = q[d];
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    float sb = -INFINITY, ov[4] = {0, 0, 0, 0};
+    double ll = 0.0;
+    wave_attend<T, PAGED>(a.kv, kvh, hd, base, qs, a.c2, j0, lim, &sb, &ll, ov);
+    ll = wave_sum_d_dpp(ll);
+    const float inv = ll == 0.0 ? 0.0f : static_cast<float>(1.0 / ll);
+    const long to = direct ? static_cast<long>(first + rr) * a.ldo + static_cast<long>(hh) * hd
+                           : (static_cast<long>(split) * a.max_rows + first + rr) * a.H + hh;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int d = lane + 64 * u;
+      if (d >= hd) continue;
+      if (direct) a.out[to + d] = ov[u] * inv;
+      else t.part[to * hd + d] = ov[u];
+    }
+    if (!direct && lane == 0) t.stat[to] = f2v{sb, static_cast<float>(ll)};
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
+template <class T, int HDP>
+void run_tiles(const AttnTask& t, bool paged, hipStream_t s) {
+  const size_t places = (static_cast<size_t>(t.r.max_rows) * (t.r.H / t.r.KV) + kTilePairs - 1) / kTilePairs + t.r.n_seqs;
+  const dim3 grid(static_cast<unsigned>(places * t.r.KV), t.tile_split.splits);
+  if (paged) attention_tiles_kernel<T, HDP, true><<<grid, kTileThreads, 0, s>>>(t);
+  else attention_tiles_kernel<T, HDP, false><<<grid, kTileThreads, 0, s>>>(t);
+}
+
+template <class T>
+void run_tiles_of(const AttnTask& t, bool paged, hipStream_t s) {
+  if (t.r.hd <= 64) run_tiles<T, 64>(t, paged, s);
+  else if (t.r.hd <= 128) run_tiles<T, 128>(t, paged, s);
+  else run_tiles<T, 256>(t, paged, s);
+}
+
+}  // namespace
+
+int launch_attention_tiles(const AttnTask& t, int qtype, bool paged, hipStream_t s) {
+  if (qtype == EF_QTYPE_F32) run_tiles_of<float>(t, paged, s);
+  else if (qtype == EF_QTYPE_F16) run_tiles_of<_Float16>(t, paged, s);
+  else run_tiles_of<__bf16>(t, paged, s);
+  EFH_HIP(hipGetLastError());
+  return EF_HIP_OK;
+}
+
+}  // namespace efh

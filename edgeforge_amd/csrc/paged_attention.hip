@@ -10,45 +10,12 @@
 namespace efh {
 namespace {
 
-// One wave per (row, query head).
-constexpr int kRowWaves = 4;
-
-template <class T, bool PAGED>
-__global__ __launch_bounds__(kRowWaves * kWave) void attention_rows_kernel(RowsArgs a) {
-  __shared__ float qs[kRowWaves][256];
-  const int row = blockIdx.x, wave = threadIdx.x / kWave, lane = threadIdx.x & (kWave - 1);
-  const int h = blockIdx.y * kRowWaves + wave;
-  const int total = min(a.row_start[a.n_seqs], a.max_rows);
-  if (row >= total || h >= a.H) return;
-  const int r = request_of(a.row_start, a.n_seqs, row), first = a.row_start[r], g = h / (a.H / a.KV);
-  int seen;
-  long base;
-  if constexpr (PAGED) {
-    seen = a.kv_len[r] - (a.row_start[r + 1] - row) + 1;
-    seen = static_cast<int>(min(static_cast<long>(seen), a.kv.table_ld << a.kv.page_shift));
-    base = r * a.kv.table_ld;
-  } else {
-    seen = row - first + 1;
-    base = first;
-  }
-  for (int d = lane; d < a.hd; d += kWave) qs[wave][d] = a.q[row * a.ldq + static_cast<long>(h) * a.hd + d];
-  float sub = -INFINITY, o[4] = {0, 0, 0, 0};
-  double l = 0.0;
-  wave_attend<T, PAGED>(a.kv, g, a.hd, base, qs[wave], a.c2, 0, seen, &sub, &l, o);
-  l = wave_sum_d_dpp(l);
-  const float inv = l == 0.0 ? 0.0f : static_cast<float>(1.0 / l);
-  float* out = a.out + row * a.ldo + static_cast<long>(h) * a.hd;
-#pragma unroll
-  for (int u = 0; u < 4; ++u)
-    if (lane + 64 * u < a.hd) out[lane + 64 * u] = o[u] * inv;
-}
-
 int check_rows(const RowsArgs& a, size_t heads, size_t KV, size_t n_seqs, size_t max_rows, size_t ldq, size_t ldo,
                float scale, const std::string& w) {
   EFH_CHECK(a.q && a.out && a.row_start, w + "null pointer");
   EFH_CHECK(heads >= 1 && heads <= 65535 && KV >= 1 && heads % KV == 0, w + "heads must be a multiple of the KV heads");
   EFH_CHECK(n_seqs >= 1 && n_seqs <= (size_t(1) << 20), w + "n_seqs must be in [1, 2^20]");
-  EFH_CHECK(max_rows <= (size_t(1) << 30), w + "max_rows too large");
+  EFH_CHECK(max_rows <= (size_t(1) << 30) / heads, w + "too many rows and heads");
   const size_t nq = heads * static_cast<size_t>(a.hd);
   EFH_CHECK(max_rows <= 1 || (ldq >= nq && ldo >= nq), w + "a row stride is shorter than its row");
   EFH_CHECK(ldq % 4 == 0 && ldo % 4 == 0 && aligned16(a.q) && aligned16(a.out),
@@ -57,39 +24,43 @@ int check_rows(const RowsArgs& a, size_t heads, size_t KV, size_t n_seqs, size_t
   return EF_HIP_OK;
 }
 
-template <bool PAGED>
-int launch_rows(const RowsArgs& a, int qtype, hipStream_t s) {
-  const dim3 grid(a.max_rows, (a.H + kRowWaves - 1) / kRowWaves);
-  const int threads = kRowWaves * kWave;
-  if (qtype == EF_QTYPE_F32) attention_rows_kernel<float, PAGED><<<grid, threads, 0, s>>>(a);
-  else if (qtype == EF_QTYPE_F16) attention_rows_kernel<_Float16, PAGED><<<grid, threads, 0, s>>>(a);
-  else attention_rows_kernel<__bf16, PAGED><<<grid, threads, 0, s>>>(a);
-  EFH_HIP(hipGetLastError());
-  return EF_HIP_OK;
-}
-
-// How a call of paged attention runs.
+// How a call of paged attention runs: the few-rows kernel for requests of up to few_most (row, head) pairs of a KV
+// head, the tiles kernel for those above, either alone where the bounds leave no request to the other.
 struct PagedPlan {
-  bool few = false;
-  int tiles = 1, splits = 1, span = 128;
+  bool few = false, tiles = false;
+  int few_most = 0, few_tiles = 1;
+  Split few_split{1, 0x40000000}, tile_split{1, 0x40000000};
   size_t bytes = 0;  // workspace
 };
-constexpr int kFewPairs = 16, kSpanStep = 128, kSpanLeast = 256, kSpanMost = 4096, kSplitWorkgroups = 1024;
+constexpr int kFewPairs = 16, kFewAlone = 64;
+constexpr int kFewStep = 128, kFewSpanLeast = 256, kFewSpanMost = 4096, kFewWorkgroups = 1024;
+constexpr int kTileStep = 64, kTileSpanLeast = 512, kTileWorkgroups = 512;
+
+// Ranges of positions so that `wgs` workgroups per range make about `want`, none shorter than `least`.
+Split split_over(size_t wgs, size_t want, size_t longest, size_t least, size_t most, size_t step) {
+  const size_t ranges = (want + wgs - 1) / wgs;
+  size_t span = std::min(std::max((longest + ranges - 1) / ranges, least), most);
+  span = std::max(span, (longest + 1023) / 1024);
+  span = (span + step - 1) / step * step;
+  return Split{static_cast<int>((longest + span - 1) / span), static_cast<int>(span)};
+}
 
 PagedPlan plan_paged(size_t H, size_t KV, size_t hd, size_t n_seqs, size_t max_rows, size_t max_new, size_t max_kv) {
   PagedPlan p;
-  const size_t pairs = std::max<size_t>(max_new, 1) * (H / KV);
-  p.few = pairs <= 64;
-  if (!p.few) return p;
-  p.tiles = static_cast<int>((pairs + kFewPairs - 1) / kFewPairs);
-  const size_t wgs = n_seqs * KV * p.tiles, want = (kSplitWorkgroups + wgs - 1) / wgs;
-  const size_t longest = std::max<size_t>(max_kv, 1);
-  size_t span = std::min<size_t>(std::max<size_t>((longest + want - 1) / want, kSpanLeast), kSpanMost);
-  span = std::max(span, (longest + 1023) / 1024);
-  span = (span + kSpanStep - 1) / kSpanStep * kSpanStep;
-  p.span = static_cast<int>(span);
-  p.splits = static_cast<int>((longest + span - 1) / span);
-  if (p.splits > 1) p.bytes = max_rows * H * p.splits * (hd + 2) * sizeof(float);
+  const size_t G = H / KV, pairs = std::max<size_t>(max_new, 1) * G, longest = std::max<size_t>(max_kv, 1);
+  p.few = pairs <= kFewAlone || n_seqs > 1;
+  p.tiles = pairs > kFewAlone;
+  const size_t few_pairs = p.tiles ? std::max<size_t>(kFewPairs, G) : pairs;
+  if (p.few) {
+    p.few_most = p.tiles ? static_cast<int>(few_pairs) : 0x7FFFFFFF;
+    p.few_tiles = static_cast<int>((few_pairs + kFewPairs - 1) / kFewPairs);
+    p.few_split = split_over(n_seqs * KV * p.few_tiles, kFewWorkgroups, longest, kFewSpanLeast, kFewSpanMost, kFewStep);
+  }
+  if (p.tiles)
+    p.tile_split = split_over((max_rows * G + kTilePairs - 1) / kTilePairs * KV + 1, kTileWorkgroups, longest, kTileSpanLeast,
+                              0x40000000, kTileStep);
+  const size_t splits = std::max(p.few_split.splits, p.tile_split.splits);
+  if (splits > 1) p.bytes = max_rows * H * splits * (hd + 2) * sizeof(float);
   return p;
 }
 
@@ -136,19 +107,22 @@ int ef_hip_paged_attention(const float* q, size_t ldq, float* out, size_t ldo, s
   const PagedPlan p = plan_paged(heads, pool->KV, pool->hd, b.n_seqs, b.max_rows, b.max_new, b.max_kv);
   EFH_CHECK(p.bytes == 0 || (ws != nullptr && ws_bytes >= p.bytes && aligned16(ws)),
             "paged_attention: the workspace must have ef_hip_paged_attention_workspace_bytes bytes, at a multiple of 16");
-  EFH_CHECK(b.n_seqs * pool->KV <= size_t(0x7FFFFFFF) / p.tiles, "paged_attention: too many requests and heads");
+  EFH_CHECK(b.n_seqs * pool->KV <= size_t(0x7FFFFFFF) / p.few_tiles, "paged_attention: too many requests and heads");
   EFH_RC(require_ready());
   if (b.max_rows == 0) return EF_HIP_OK;
-  if (!p.few) return launch_rows<true>(a, pool->qtype, pick(stream));
   AttnTask t{};
   t.r = a;
-  t.tiles = p.tiles;
-  t.few_most = 0x7FFFFFFF;
-  t.s.splits = p.splits;
-  t.s.span = p.span;
-  t.s.part = static_cast<float*>(ws);
-  t.s.stat = reinterpret_cast<f2v*>(t.s.part + b.max_rows * heads * p.splits * pool->hd);
-  return launch_attention_few(t, pool->qtype, pick(stream));
+  t.few_split = p.few_split;
+  t.tile_split = p.tile_split;
+  t.tiles = p.few_tiles;
+  t.few_most = p.few_most;
+  const size_t splits = std::max(p.few_split.splits, p.tile_split.splits);
+  t.part = static_cast<float*>(ws);
+  t.stat = reinterpret_cast<f2v*>(t.part + b.max_rows * heads * splits * pool->hd);
+  hipStream_t s = pick(stream);
+  if (p.tiles) EFH_RC(launch_attention_tiles(t, pool->qtype, true, s));
+  if (p.few) EFH_RC(launch_attention_few(t, pool->qtype, s));
+  return splits > 1 ? launch_attention_join(t, s) : EF_HIP_OK;
 }
 
 size_t ef_hip_packed_attention_workspace_bytes(size_t heads, size_t KV, size_t hd, int qtype, size_t n_seqs,
@@ -185,7 +159,10 @@ int ef_hip_packed_attention(const float* q, size_t ldq, const void* k, size_t ld
   (void)ws, (void)ws_bytes;
   EFH_RC(require_ready());
   if (max_rows == 0) return EF_HIP_OK;
-  return launch_rows<false>(a, qtype, pick(stream));
+  AttnTask t{};
+  t.r = a;
+  t.tile_split = Split{1, 0x40000000};
+  return launch_attention_tiles(t, qtype, false, pick(stream));
 }
 
 }  // extern "C"
