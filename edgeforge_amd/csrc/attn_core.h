@@ -140,10 +140,13 @@ __device__ __forceinline__ void split8(const float (&x)[8], u4v (&part)[Parts<T>
   for (int i = 0; i < 4; ++i) {
     float a = x[2 * i], b = x[2 * i + 1];
     if constexpr (std::is_same_v<T, _Float16>) {
-      const h2v hi = __builtin_convertvector((f2v{a, b}), h2v);
-      part[0][i] = __builtin_bit_cast(uint32_t, hi);
-      const h2v lo = __builtin_convertvector((f2v{a - static_cast<float>(hi[0]), b - static_cast<float>(hi[1])}), h2v);
-      part[1][i] = __builtin_bit_cast(uint32_t, lo);
+      const uint32_t hi = __builtin_bit_cast(uint32_t, __builtin_convertvector((f2v{a, b}), h2v));
+      part[0][i] = hi;
+      // what the halves left: x - half in one instruction, the half widened on the way (the conversion above has
+      // read a and b, so their results are there)
+      asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(a) : "v"(hi), "v"(a));
+      asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(b) : "v"(hi), "v"(b));
+      part[1][i] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f2v{a, b}), h2v));
     } else {
       part[0][i] = high_halves(a, b);
       a -= __uint_as_float(__float_as_uint(a) & 0xFFFF0000u);

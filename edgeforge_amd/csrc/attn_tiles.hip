@@ -59,26 +59,47 @@ __device__ __forceinline__ int request_of_place(const RowsArgs& a, long x) {
   return __builtin_amdgcn_readfirstlane(lo);
 }
 
-template <class T, int HDP, bool PAGED>
+template <class T, int HDP>
 struct TileShape {
   static constexpr bool F32 = sizeof(T) == 4;
   static constexpr int BN = HDP == 256 || (F32 && HDP >= 128) ? 32 : 64;  // positions of a tile
-  static constexpr int PLANES = F32 ? 3 : 1;                    // 16-bit planes of a key or value
-  static constexpr int LDK = HDP + 8, LDV = HDP + 16;           // 16-bit values between rows: no bank conflicts
-  static constexpr int UNITS = BN * HDP / 8 / kTileThreads;     // groups of 8 values that a thread stages
+  static constexpr int PLANES = F32 ? 3 : 1;                              // 16-bit planes of a key or value
+  static constexpr int CHUNKS = HDP / 8;                                  // 16-byte chunks of a row
+  static constexpr int PLANE = BN * HDP;                                  // 16-bit values of a plane
+  static constexpr int BUFFERS = F32 ? 1 : 2;
+  static constexpr int UNITS = PLANE / 8 / kTileThreads;                  // chunks that a thread brings of keys, and of values
 };
+
+// Rows lie in LDS without padding (a DMA instruction writes 1 KB in one piece), chunk c of row r at place c ^ (r & 7)
+// of the keys' row, c ^ 2 (r & 3) of the values': eight lanes that read a chunk of eight rows, and sixteen that read
+// 32 bytes of four rows, then hit different banks.
+__device__ __forceinline__ int k_place(int chunk, int row) { return chunk ^ (row & 7); }
+__device__ __forceinline__ int v_place(int chunk, int row) { return chunk ^ ((row & 3) << 1); }
+
+// 16 bytes per lane from src to LDS at dst + 16 lane, asynchronously (vmcnt).  As asm because the compiler, seeing
+// such a copy, waits for it before every later LDS read; the kernel waits for its tiles itself.  No register is
+// written but m0, which the compiler sets anew before each use.
+__device__ __forceinline__ void tile_dma16(uint32_t dst, const void* src) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(dst), "v"(src) : "memory");
+}
+// This wave's copies arrived and its LDS accesses done, then the barrier.
+__device__ __forceinline__ void tile_barrier() {
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
 
 template <class T, int HDP, bool PAGED>
 __global__ __launch_bounds__(kTileThreads, HDP == 64 && sizeof(T) == 2 ? 3 : HDP <= 128 ? 2 : 1) void attention_tiles_kernel(AttnTask t) {
-  using Sh = TileShape<T, HDP, PAGED>;
+  using Sh = TileShape<T, HDP>;
   constexpr bool F32 = Sh::F32;
-  constexpr int BN = Sh::BN, SUB = BN / 32, PLANES = Sh::PLANES, LDK = Sh::LDK, LDV = Sh::LDV, UNITS = Sh::UNITS;
-  constexpr int KK = HDP / 16, DT = HDP / 32, NS = Parts<T>::N;
+  constexpr int BN = Sh::BN, SUB = BN / 32, PLANES = Sh::PLANES, CHUNKS = Sh::CHUNKS, PLANE = Sh::PLANE, UNITS = Sh::UNITS;
+  constexpr int BUFFERS = Sh::BUFFERS, KK = HDP / 16, DT = HDP / 32, NS = Parts<T>::N;
   constexpr float OFFSET = Parts<T>::kSubOffset;
-  __shared__ __attribute__((aligned(16))) uint16_t ks[PLANES * BN * LDK];
-  __shared__ __attribute__((aligned(16))) uint16_t vs[PLANES * BN * LDV];
-  __shared__ uint32_t ok_s[BN / 4];  // a byte per position: whether a page holds it
-  __shared__ int lost_s;             // some tile so far had a position without a page
+  __shared__ __attribute__((aligned(1024))) uint16_t ks[BUFFERS][PLANES * PLANE];
+  __shared__ __attribute__((aligned(1024))) uint16_t vs[BUFFERS][PLANES * PLANE];
+  __shared__ uint32_t ok_s[2][BN / 4];  // a byte per position: whether a page holds it
+  __shared__ int lost_s;                      // some tile so far had a position without a page
 
   const RowsArgs& a = t.r;
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid & (kWave - 1);
@@ -148,44 +169,79 @@ __global__ __launch_bounds__(kTileThreads, HDP == 64 && sizeof(T) == 2 ? 3 : HDP
     }
   }
 
-  // ---- staging -------------------------------------------------------------------------------------------
-  constexpr int ROW_UNITS = HDP / 8, WORDS = F32 ? 2 : 1;
-  u4v kr[UNITS][WORDS], vr[UNITS][WORDS];
-  bool real[UNITS];
-  const int unit_col = 8 * (tid % ROW_UNITS), unit_row = tid / ROW_UNITS;  // unit u: row unit_row + u * 256 / ROW_UNITS
-  const bool in_row = unit_col < hd;
-  const T *kp = static_cast<const T*>(a.kv.k), *vp = static_cast<const T*>(a.kv.v);
-  auto fetch = [&](int c) {
+  // ---- bringing tiles ------------------------------------------------------------------------------------
+  // Unit u of a thread: the chunk at place (tid % CHUNKS) of row tid / CHUNKS + u * 256 / CHUNKS.  16-bit tiles go to
+  // LDS by DMA, a tile ahead, in two buffers; FP32 ones through registers, where they are split.  Rows past j1
+  // repeat the last one, rows without a page the pool's first, dims past hd the row's last ones: all are masked
+  // or multiplied by zero.
+  constexpr int ROWS = kTileThreads / CHUNKS, WORDS = F32 ? 2 : 1;
+  const int my_place = tid % CHUNKS, my_row = tid / CHUNKS;
+  const int k_col = min(8 * k_place(my_place, my_row), hd - 8), v_col = min(8 * v_place(my_place, my_row), hd - 8);
+  const T *kp = static_cast<const T*>(a.kv.k) + k_col, *vp = static_cast<const T*>(a.kv.v) + (F32 ? k_col : v_col);
+  static_assert(ROWS % 8 == 0, "a thread's rows share their places");
+  int page[UNITS];  // of the next tile's rows
+  auto look_up = [&](int c) {
+    if constexpr (PAGED) {
+#pragma unroll
+      for (int u = 0; u < UNITS; ++u) page[u] = a.kv.table[base + (min(c + my_row + u * ROWS, j1 - 1) >> a.kv.page_shift)];
+    }
+  };
+  u4v kr[F32 ? UNITS : 1][WORDS], vr[F32 ? UNITS : 1][WORDS];
+  const uint32_t k_lds = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) void*)ks)) + 1024 * wave;
+  const uint32_t v_lds = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) void*)vs)) + 1024 * wave;
+  auto bring = [&](int c, int buf, int ok_buf) {
 #pragma unroll
     for (int u = 0; u < UNITS; ++u) {
-      const int j = c + unit_row + u * (kTileThreads / ROW_UNITS);
-      long ko = 0, vo = 0;
-      real[u] = j < j1 && kv_offset<PAGED>(a.kv, kvh, hd, base, j, &ko, &vo);
-#pragma unroll
-      for (int w = 0; w < WORDS; ++w) kr[u][w] = vr[u][w] = u4v{0, 0, 0, 0};
-      if (real[u] && in_row) {
+      const int r = my_row + u * ROWS, j = min(c + r, j1 - 1);
+      long ko, vo;
+      if constexpr (PAGED) {
+        const bool real = static_cast<uint32_t>(page[u]) < static_cast<uint32_t>(a.kv.n_pages);
+        ko = vo = real ? page[u] * a.kv.page_stride + ((static_cast<long>(kvh) << a.kv.page_shift) + (j & ((1 << a.kv.page_shift) - 1))) * hd : 0;
+        if (my_place == 0) {
+          reinterpret_cast<uint8_t*>(ok_s[ok_buf])[r] = real;
+          if (!real) lost_s = 1;
+        }
+      } else {
+        ko = (base + j) * a.kv.ldk + static_cast<long>(kvh) * hd;
+        vo = (base + j) * a.kv.ldv + static_cast<long>(kvh) * hd;
+      }
+      if constexpr (F32) {
 #pragma unroll
         for (int w = 0; w < WORDS; ++w) {
-          kr[u][w] = *reinterpret_cast<const u4v*>(kp + ko + unit_col + 4 * w);
-          vr[u][w] = *reinterpret_cast<const u4v*>(vp + vo + unit_col + 4 * w);
+          kr[u][w] = *reinterpret_cast<const u4v*>(kp + ko + 4 * w);
+          vr[u][w] = *reinterpret_cast<const u4v*>(vp + vo + 4 * w);
+        }
+      } else {
+        tile_dma16(k_lds + (buf * PLANE + u * 8 * kTileThreads) * 2, kp + ko);
+        tile_dma16(v_lds + (buf * PLANE + u * 8 * kTileThreads) * 2, vp + vo);
+      }
+    }
+  };
+  auto put = [&]() {  // FP32: the registers' rows into LDS, split
+    if constexpr (F32) {
+#pragma unroll
+      for (int u = 0; u < UNITS; ++u) {
+        const int r = my_row + u * ROWS, chunk = k_place(my_place, my_row);
+#pragma unroll
+        for (int which = 0; which < 2; ++which) {
+          const u4v(&x)[WORDS] = which ? vr[u] : kr[u];
+          float f[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(x[i / 4][i % 4]);
+          u4v part[3];
+          split8<float>(f, part);
+          uint16_t* dst = which ? vs[0] + r * HDP + 8 * v_place(chunk, r) : ks[0] + r * HDP + 8 * k_place(chunk, r);
+#pragma unroll
+          for (int p = 0; p < 3; ++p) *reinterpret_cast<u4v*>(dst + p * PLANE) = part[p];
         }
       }
     }
   };
-  auto put = [&](uint16_t* dst, int ld, const u4v (&x)[WORDS], int r) {
-    if constexpr (F32) {
-      float f[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(x[i / 4][i % 4]);
-      u4v part[3];
-      split8<float>(f, part);
-#pragma unroll
-      for (int p = 0; p < 3; ++p) *reinterpret_cast<u4v*>(dst + (p * BN + r) * ld + unit_col) = part[p];
-    } else {
-      *reinterpret_cast<u4v*>(dst + r * ld + unit_col) = x[0];
-    }
-  };
   if (tid == 0) lost_s = 0;
+  __syncthreads();
+  // this lane's reads: keys' row col, chunk 2 k + h; values' rows 4 h + lane % 16 / 4, dims 16 (lane / 16 % 2) + 4 (lane % 4)
+  const int vq = (lane & 15) / 4, vchunk = 2 * (lane >> 4 & 1) + (lane & 3) / 2;
+  const int k_at = col * HDP, v_at = (4 * h + vq) * HDP + 4 * (lane & 1);
 
   f16v o[DT];
 #pragma unroll
@@ -193,42 +249,45 @@ __global__ __launch_bounds__(kTileThreads, HDP == 64 && sizeof(T) == 2 ? 3 : HDP
 #pragma unroll
     for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
   float sub = -INFINITY, l = 0.0f;
-  if (j0 < j1) fetch(j0);
+  if (j0 < j1) {
+    look_up(j0);
+    bring(j0, 0, 0);
+    look_up(j0 + BN);
+  }
+  int turn = 0;
   for (int c = j0; c < j1; c += BN) {
-    __syncthreads();  // the tile before is used
-#pragma unroll
-    for (int u = 0; u < UNITS; ++u) {
-      const int r = unit_row + u * (kTileThreads / ROW_UNITS);
-      put(ks, LDK, kr[u], r);
-      put(vs, LDV, vr[u], r);
-      if constexpr (PAGED) {
-        if (unit_col == 0) {
-          reinterpret_cast<uint8_t*>(ok_s)[r] = real[u];
-          if (!real[u] && c + r < j1) lost_s = 1;
-        }
-      }
+    if constexpr (F32) {
+      if (c != j0) tile_barrier();  // the tile before is used
+      put();
     }
-    __syncthreads();
-    if (c + BN < j1) fetch(c + BN);
+    tile_barrier();  // the tile is there, and the buffer of the tile before is free
+    const int now = F32 ? 0 : turn, ok_now = turn;
+    turn ^= 1;
+    if (c + BN < j1) {
+      bring(c + BN, F32 ? 0 : turn, turn);
+      look_up(c + 2 * BN);
+    }
     if (!busy) continue;
+    const uint16_t *kt = ks[now] + k_at, *vt = vs[now] + v_at;
 
     f16v sc[SUB];
 #pragma unroll
     for (int s = 0; s < SUB; ++s) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) sc[s][i] = 0.0f;
+      u4v kf[KK][PLANES];
 #pragma unroll
-      for (int k = 0; k < KK; ++k) {
-        u4v kf[PLANES];
+      for (int k = 0; k < KK; ++k)
 #pragma unroll
         for (int p = 0; p < PLANES; ++p)
-          kf[p] = *reinterpret_cast<const u4v*>(ks + (p * BN + 32 * s + col) * LDK + 16 * k + 8 * h);
+          kf[k][p] = *reinterpret_cast<const u4v*>(kt + p * PLANE + 32 * s * HDP + 8 * k_place(2 * k + h, col));
+#pragma unroll
+      for (int k = 0; k < KK; ++k)
 #pragma unroll
         for (int sum = NS - 1; sum >= 0; --sum)  // the small products first
 #pragma unroll
           for (int p = 0; p < PLANES; ++p)
-            if (sum - p >= 0) sc[s] = mfma32<T>(kf[p], qp[k][sum - p], sc[s]);
-      }
+            if (sum - p >= 0) sc[s] = mfma32<T>(kf[k][p], qp[k][sum - p], sc[s]);
     }
     if (c + BN > all_see) {
 #pragma unroll
@@ -243,7 +302,7 @@ __global__ __launch_bounds__(kTileThreads, HDP == 64 && sizeof(T) == 2 ? 3 : HDP
         for (int s = 0; s < SUB; ++s)
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
-            const uint32_t w = ok_s[8 * s + 2 * q + h];
+            const uint32_t w = ok_s[ok_now][8 * s + 2 * q + h];
 #pragma unroll
             for (int i = 0; i < 4; ++i)
               if (!(w >> (8 * i) & 255)) sc[s][4 * q + i] = -INFINITY;
@@ -283,9 +342,9 @@ __global__ __launch_bounds__(kTileThreads, HDP == 64 && sizeof(T) == 2 ? 3 : HDP
           u4v vf[PLANES];
 #pragma unroll
           for (int pl = 0; pl < PLANES; ++pl) {
-            uint16_t* at = vs + (pl * BN + 32 * s + 16 * half + 4 * h + (lane & 15) / 4) * LDV + 32 * d + 16 * (lane >> 4 & 1) + 4 * (lane & 3);
+            uint16_t* at = const_cast<uint16_t*>(vt) + pl * PLANE + (32 * s + 16 * half) * HDP + 8 * v_place(4 * d + vchunk, vq);
             const s4v lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4v)at);
-            const s4v hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4v)(at + 8 * LDV));
+            const s4v hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4v)(at + 8 * HDP));
             const u2v lw = __builtin_bit_cast(u2v, lo), hw = __builtin_bit_cast(u2v, hi);
             vf[pl] = u4v{lw[0], lw[1], hw[0], hw[1]};
           }
@@ -324,8 +383,8 @@ __global__ __launch_bounds__(kTileThreads, HDP == 64 && sizeof(T) == 2 ? 3 : HDP
   }
   uint64_t todo = __ballot(bad && active);
   todo = (todo | todo >> 32) & 0xFFFFFFFFull;
-  __syncthreads();  // the last tile is used
-  float* qs = reinterpret_cast<float*>(ks) + wave * HDP;
+  tile_barrier();  // the last tile is used
+  float* qs = reinterpret_cast<float*>(ks[0]) + wave * HDP;
   for (; todo; todo &= todo - 1) {
     const int who = __ffsll(static_cast<unsigned long long>(todo)) - 1;
     const int rr = __shfl(row, who, kWave), hh = __shfl(head, who, kWave), lim = min(j1, __shfl(seen, who, kWave));

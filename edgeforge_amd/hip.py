@@ -10,7 +10,7 @@ import ctypes as C
 import numpy as np
 
 from . import _lib as L
-from ._lib import BF16, F16, F32, Q4_0, Q8_0, call, lib
+from ._lib import BF16, F16, F32, Q4_0, Q8_0, call, check, lib
 
 __all__ = ["DeviceArray", "Weight", "Stream", "Event", "init", "row_bytes", "matvec", "matvec_jobs",
            "matvec_residual", "matvec_swiglu", "matvec_jobs_rmsnorm", "quantize", "rows_f32", "argmax", "sampler_exp",
@@ -261,13 +261,14 @@ class PagePool:
         self.k, self.v = own
         sync()
         self.c = L.ef_hip_page_pool(_p(self.k), _p(self.v), qtype, n_pages, page_size, KV, hd, self.page_stride)
+        self.ref = C.byref(self.c)
 
 
 def page_plan(cached, new, seqs: int, page_size: int, n_pages: int, table, table_ld: int, free, n_free, n_free_out, kv_len,
               row_start, pos, slot, max_rows: int, status, stream=None) -> None:
     """One step's block tables and slot maps from the requests' lengths (ef_hip_page_plan)."""
-    call("ef_hip_page_plan", _p(cached), _p(new), seqs, page_size, n_pages, _p(table), table_ld, _p(free), _p(n_free),
-         _p(n_free_out), _p(kv_len), _p(row_start), _p(pos), _p(slot), max_rows, _p(status), _s(stream))
+    check(lib().ef_hip_page_plan(cached.ptr, new.ptr, seqs, page_size, n_pages, table.ptr, table_ld, free.ptr, n_free.ptr,
+                                 n_free_out.ptr, kv_len.ptr, row_start.ptr, pos.ptr, slot.ptr, max_rows, status.ptr, _s(stream)))
 
 
 def rope_tables(theta: float, hd: int, n_pos: int) -> tuple[DeviceArray, DeviceArray]:
@@ -277,24 +278,27 @@ def rope_tables(theta: float, hd: int, n_pos: int) -> tuple[DeviceArray, DeviceA
     return cos, sin
 
 
+# q, k, v and outputs below may be raw device addresses (rows inside a wider buffer), as in matvec_jobs.
 def rope_append(q, ldq: int, q_out, ldqo: int, heads: int, k, ldk: int, v, ldv: int, rows: int, pos, cos, sin, n_pos: int,
                 slot, pool: PagePool, k_out=None, ldko: int = 0, stream=None) -> None:
     """RoPE on queries and keys, keys and values stored into the pool (ef_hip_rope_append)."""
-    call("ef_hip_rope_append", _p(q), ldq, _p(q_out), ldqo, heads, _p(k), ldk, _p(k_out), ldko, _p(v), ldv, rows, _p(pos),
-         _p(cos), _p(sin), n_pos, _p(slot), C.byref(pool.c), _s(stream))
+    check(lib().ef_hip_rope_append(q if type(q) is int else q.ptr, ldq, q_out if type(q_out) is int else q_out.ptr, ldqo, heads,
+                                   k if type(k) is int else k.ptr, ldk, _p(k_out), ldko, v if type(v) is int else v.ptr, ldv, rows,
+                                   pos.ptr, cos.ptr, sin.ptr, n_pos, slot.ptr, pool.ref, _s(stream)))
 
 
 def paged_attention_workspace_bytes(heads: int, pool: PagePool, seqs: int, max_rows: int, max_new: int,
                                     max_kv: int) -> int:
-    return lib().ef_hip_paged_attention_workspace_bytes(heads, C.byref(pool.c), seqs, max_rows, max_new, max_kv)
+    return lib().ef_hip_paged_attention_workspace_bytes(heads, pool.ref, seqs, max_rows, max_new, max_kv)
 
 
 def paged_attention(q, ldq: int, out, ldo: int, heads: int, pool: PagePool, table, table_ld: int, row_start, kv_len,
                     seqs: int, max_rows: int, max_new: int, max_kv: int, scale: float, ws=None, stream=None) -> None:
     """Attention of each request's new rows over its pages (ef_hip_paged_attention)."""
-    b = L.ef_hip_paged_batch(_p(row_start), _p(kv_len), _p(table), table_ld, seqs, max_rows, max_new, max_kv)
-    call("ef_hip_paged_attention", _p(q), ldq, _p(out), ldo, heads, C.byref(pool.c), C.byref(b), scale, _p(ws),
-         ws.nbytes if ws is not None else 0, _s(stream))
+    b = L.ef_hip_paged_batch(row_start.ptr, kv_len.ptr, table.ptr, table_ld, seqs, max_rows, max_new, max_kv)
+    check(lib().ef_hip_paged_attention(q if type(q) is int else q.ptr, ldq, out if type(out) is int else out.ptr, ldo, heads, pool.ref,
+                                       C.byref(b), scale, ws.ptr if ws is not None else None, ws.nbytes if ws is not None else 0,
+                                       _s(stream)))
 
 
 def packed_attention_workspace_bytes(heads: int, KV: int, hd: int, qtype: int, seqs: int, max_rows: int) -> int:
@@ -304,5 +308,7 @@ def packed_attention_workspace_bytes(heads: int, KV: int, hd: int, qtype: int, s
 def packed_attention(q, ldq: int, k, ldk: int, v, ldv: int, qtype: int, out, ldo: int, heads: int, KV: int, hd: int, row_start,
                      seqs: int, max_rows: int, scale: float, ws=None, stream=None) -> None:
     """Causal attention over packed prompts (ef_hip_packed_attention)."""
-    call("ef_hip_packed_attention", _p(q), ldq, _p(k), ldk, _p(v), ldv, qtype, _p(out), ldo, heads, KV, hd, _p(row_start),
-         seqs, max_rows, scale, _p(ws), ws.nbytes if ws is not None else 0, _s(stream))
+    check(lib().ef_hip_packed_attention(q if type(q) is int else q.ptr, ldq, k if type(k) is int else k.ptr, ldk,
+                                        v if type(v) is int else v.ptr, ldv, qtype, out if type(out) is int else out.ptr, ldo, heads,
+                                        KV, hd, row_start.ptr, seqs, max_rows, scale, ws.ptr if ws is not None else None,
+                                        ws.nbytes if ws is not None else 0, _s(stream)))
