@@ -70,11 +70,17 @@ struct TileShape {
   static constexpr int UNITS = PLANE / 8 / kTileThreads;                  // chunks that a thread brings of keys, and of values
 };
 
-// Rows lie in LDS without padding (a DMA instruction writes 1 KB in one piece), chunk c of row r at place c ^ (r & 7)
-// of the keys' row, c ^ 2 (r & 3) of the values': eight lanes that read a chunk of eight rows, and sixteen that read
-// 32 bytes of four rows, then hit different banks.
-__device__ __forceinline__ int k_place(int chunk, int row) { return chunk ^ (row & 7); }
-__device__ __forceinline__ int v_place(int chunk, int row) { return chunk ^ ((row & 3) << 1); }
+// Rows lie in LDS without padding (a DMA instruction writes 1 KB in one piece), their 16-byte chunks in another order in
+// each row, so that what one LDS cycle serves hits all 64 banks: sixteen lanes that read a chunk of sixteen rows
+// (keys), and 32 that read 64 bytes of four rows (values).  Rows of 128 bytes are half the banks wide.
+template <int CHUNKS>
+__device__ __forceinline__ int k_place(int chunk, int row) {
+  return chunk ^ (CHUNKS == 8 ? row >> 1 & 7 : row & (CHUNKS == 16 ? 15 : 7));
+}
+template <int CHUNKS>
+__device__ __forceinline__ int v_place(int chunk, int row) {
+  return chunk ^ (CHUNKS == 8 ? (row & 2) << 1 : (row & 3) << 2);
+}
 
 // 16 bytes per lane from src to LDS at dst + 16 lane, asynchronously (vmcnt).  As asm because the compiler, seeing
 // such a copy, waits for it before every later LDS read; the kernel waits for its tiles itself.  No register is
@@ -176,9 +182,9 @@ __global__ __launch_bounds__(kTileThreads, HDP == 64 && sizeof(T) == 2 ? 3 : HDP
   // or multiplied by zero.
   constexpr int ROWS = kTileThreads / CHUNKS, WORDS = F32 ? 2 : 1;
   const int my_place = tid % CHUNKS, my_row = tid / CHUNKS;
-  const int k_col = min(8 * k_place(my_place, my_row), hd - 8), v_col = min(8 * v_place(my_place, my_row), hd - 8);
+  const int k_col = min(8 * k_place<CHUNKS>(my_place, my_row), hd - 8), v_col = min(8 * v_place<CHUNKS>(my_place, my_row), hd - 8);
   const T *kp = static_cast<const T*>(a.kv.k) + k_col, *vp = static_cast<const T*>(a.kv.v) + (F32 ? k_col : v_col);
-  static_assert(ROWS % 8 == 0, "a thread's rows share their places");
+  static_assert(ROWS % (CHUNKS == 32 ? 8 : 16) == 0, "a thread's rows share their places");
   int page[UNITS];  // of the next tile's rows
   auto look_up = [&](int c) {
     if constexpr (PAGED) {
@@ -221,7 +227,7 @@ __global__ __launch_bounds__(kTileThreads, HDP == 64 && sizeof(T) == 2 ? 3 : HDP
     if constexpr (F32) {
 #pragma unroll
       for (int u = 0; u < UNITS; ++u) {
-        const int r = my_row + u * ROWS, chunk = k_place(my_place, my_row);
+        const int r = my_row + u * ROWS, chunk = k_place<CHUNKS>(my_place, my_row);
 #pragma unroll
         for (int which = 0; which < 2; ++which) {
           const u4v(&x)[WORDS] = which ? vr[u] : kr[u];
@@ -230,7 +236,7 @@ __global__ __launch_bounds__(kTileThreads, HDP == 64 && sizeof(T) == 2 ? 3 : HDP
           for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(x[i / 4][i % 4]);
           u4v part[3];
           split8<float>(f, part);
-          uint16_t* dst = which ? vs[0] + r * HDP + 8 * v_place(chunk, r) : ks[0] + r * HDP + 8 * k_place(chunk, r);
+          uint16_t* dst = which ? vs[0] + r * HDP + 8 * v_place<CHUNKS>(chunk, r) : ks[0] + r * HDP + 8 * k_place<CHUNKS>(chunk, r);
 #pragma unroll
           for (int p = 0; p < 3; ++p) *reinterpret_cast<u4v*>(dst + p * PLANE) = part[p];
         }
@@ -280,7 +286,7 @@ __global__ __launch_bounds__(kTileThreads, HDP == 64 && sizeof(T) == 2 ? 3 : HDP
       for (int k = 0; k < KK; ++k)
 #pragma unroll
         for (int p = 0; p < PLANES; ++p)
-          kf[k][p] = *reinterpret_cast<const u4v*>(kt + p * PLANE + 32 * s * HDP + 8 * k_place(2 * k + h, col));
+          kf[k][p] = *reinterpret_cast<const u4v*>(kt + p * PLANE + 32 * s * HDP + 8 * k_place<CHUNKS>(2 * k + h, col));
 #pragma unroll
       for (int k = 0; k < KK; ++k)
 #pragma unroll
@@ -342,7 +348,7 @@ __global__ __launch_bounds__(kTileThreads, HDP == 64 && sizeof(T) == 2 ? 3 : HDP
           u4v vf[PLANES];
 #pragma unroll
           for (int pl = 0; pl < PLANES; ++pl) {
-            uint16_t* at = const_cast<uint16_t*>(vt) + pl * PLANE + (32 * s + 16 * half) * HDP + 8 * v_place(4 * d + vchunk, vq);
+            uint16_t* at = const_cast<uint16_t*>(vt) + pl * PLANE + (32 * s + 16 * half) * HDP + 8 * v_place<CHUNKS>(4 * d + vchunk, vq);
             const s4v lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4v)at);
             const s4v hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4v)(at + 8 * HDP));
             const u2v lw = __builtin_bit_cast(u2v, lo), hw = __builtin_bit_cast(u2v, hi);
