@@ -209,7 +209,17 @@ struct AttnTask {
   Split few_split, tile_split;
   float* part;  // [splits][rows * H][hd]
   f2v* stat;    // [splits][rows * H]: sub, l
+  int* count;   // [rows * H]: ranges that hold sums (one: the output is already there); null where nothing is split
+  int group;       // H / KV
+  uint32_t magic;  // ceil(2^32 / group)
+  // pair / group: the product's high half is the quotient or one more (its error is below pair group / 2^32 < group)
+  __device__ __forceinline__ int row_of(int pair) const {
+    if (group == 1) return pair;
+    const int q = static_cast<int>(__umulhi(static_cast<uint32_t>(pair), magic));
+    return q - (static_cast<int64_t>(q) * group > pair);
+  }
   int tiles;     // few-rows kernel: workgroups per (request, KV head) along its rows
+  bool few_wide; // few-rows kernel: 32 (row, head) pairs to a workgroup, not 16
   int few_most;  // (row, head) pairs of a KV head up to which a request is the few-rows kernel's, not the tiles kernel's
 };
 

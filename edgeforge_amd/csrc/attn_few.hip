@@ -23,9 +23,11 @@ namespace {
 constexpr int kFewWaves = 4;
 
 template <class T, int HDP, int NT, bool WIDE>
-__global__ __launch_bounds__(kFewWaves * kWave, HDP == 256 ? 1 : (HDP == 64 ? 3 : 2) - !WIDE) void attention_few_kernel(AttnTask t) {
+__global__ __launch_bounds__(kFewWaves * kWave, HDP == 256 ? 1 : (HDP == 64 && NT == 1 ? 3 : 2) - !WIDE) void attention_few_kernel(AttnTask t) {
   constexpr bool F32 = sizeof(T) == 4;
-  constexpr int KT = F32 ? 16 : 32, TILES = KT / 16, DP = HDP / 16;
+  // positions of a step, in matrix tiles of 16 (twice as many, 16 KB a step and wave at hd = 64, cost more occupancy
+  // than they gained: 41 requests, 39 of them with one row, 54 -> 61 us)
+  constexpr int TILES = F32 ? 1 : 2, KT = 16 * TILES, DP = HDP / 16;
   constexpr int KW = F32 ? HDP / 16 : HDP / 32;  // 16-byte pieces of a key row in a lane
   constexpr int VROWS = 4 * TILES, VW = F32 ? DP / 4 : DP * 2 / 16 + (DP == 4);  // value rows of a lane, 16-byte pieces each (8 bytes for 4 halves)
   constexpr float OFFSET = F32 ? 0.0f : Parts<T>::kSubOffset;
@@ -36,12 +38,8 @@ __global__ __launch_bounds__(kFewWaves * kWave, HDP == 256 ? 1 : (HDP == 64 ? 3 
   const RowsArgs& a = t.r;
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid & (kWave - 1);
   const int m = lane & 15, g4 = lane >> 4;
-  const int split = blockIdx.y;
-  int id = blockIdx.x;
-  const int kvh = id % a.KV;
-  id /= a.KV;
-  const int tile0 = id % t.tiles, req = id / t.tiles;
-  const int hd = a.hd, G = a.H / a.KV;
+  const int req = blockIdx.x, kvh = blockIdx.y, split = blockIdx.z / t.tiles, tile0 = blockIdx.z - split * t.tiles;
+  const int hd = a.hd, G = t.group;
   const int first = a.row_start[req], n = min(a.row_start[req + 1], a.max_rows) - first;
   const long base = req * a.kv.table_ld;
   const int kv_len = a.kv_len[req];
@@ -60,72 +58,53 @@ __global__ __launch_bounds__(kFewWaves * kWave, HDP == 256 ? 1 : (HDP == 64 ? 3 
   for (int i = 0; i < KW; ++i) kd[i] = F32 ? min(16 * i + 4 * g4, hd - 4) : min(32 * i + 8 * g4, hd - 8);
 #pragma unroll
   for (int i = 0; i < VW; ++i) vd[i] = F32 ? min(m * DP + 4 * i, hd - 4) : DP == 4 ? min(m * DP, hd - 4) : min(m * DP + 8 * i, hd - 8);
+  uint32_t kb[KW], vb[VW];  // byte offsets from the first of 16 rows (wide pages: rows of a tile follow each other)
+#pragma unroll
+  for (int i = 0; i < KW; ++i) kb[i] = (m * hd + kd[i]) * sizeof(T);
+#pragma unroll
+  for (int i = 0; i < VW; ++i) vb[i] = (4 * g4 * hd + vd[i]) * sizeof(T);
 
   for (int tile = tile0; tile * PAIRS < n * G; tile += t.tiles) {
-    // ---- queries -------------------------------------------------------------------------------------
-    constexpr int NS = F32 ? 1 : Parts<T>::N;
-    f4v qf[F32 ? NT : 1][KW];
-    u4v qp[F32 ? 1 : NT][KW][NS];
-    float c2[NT];
+    // ---- queries' raw values, then the first step's rows: all in flight together ------------------------------
+    constexpr int NS = F32 ? 1 : Parts<T>::N, QW = F32 ? 1 : 2;
+    f4v qf[NT][KW][QW];
     int seen[NT];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const int pair = tile * PAIRS + 16 * nt + m, row = pair / G, head = kvh * G + pair - row * G;
+      const int pair = tile * PAIRS + 16 * nt + m, row = t.row_of(pair), head = kvh * G + pair - row * G;
       const bool active = row < n;
       seen[nt] = active ? min(before + row + 1, kv) : 0;
       const float* q = a.q + (first + (active ? row : 0)) * a.ldq + static_cast<long>(active ? head : kvh * G) * hd;
-      c2[nt] = a.c2;
-      if constexpr (F32) {
 #pragma unroll
-        for (int i = 0; i < KW; ++i) {
-          qf[nt][i] = *reinterpret_cast<const f4v*>(q + kd[i]);
-          if (16 * i + 4 * g4 >= hd) qf[nt][i] = f4v{0, 0, 0, 0};
-        }
-      } else {
-        float x[KW][8], top = 0.0f;
+      for (int i = 0; i < KW; ++i)
 #pragma unroll
-        for (int i = 0; i < KW; ++i) {
-          load8(q + kd[i], x[i]);
-          if (32 * i + 8 * g4 >= hd) {
-#pragma unroll
-            for (int u = 0; u < 8; ++u) x[i][u] = 0.0f;
-          }
-#pragma unroll
-          for (int u = 0; u < 8; ++u) top = fmaxf(top, fabsf(x[i][u]));
-        }
-        if constexpr (std::is_same_v<T, _Float16>) {
-          const int e = query_exponent(column_max(top));
-          c2[nt] = ldexpf(c2[nt], -e);
-#pragma unroll
-          for (int i = 0; i < KW; ++i)
-#pragma unroll
-            for (int u = 0; u < 8; ++u) x[i][u] = ldexpf(x[i][u], e);
-        }
-#pragma unroll
-        for (int i = 0; i < KW; ++i) split8<T>(x[i], qp[nt][i]);
-      }
+        for (int w = 0; w < QW; ++w) qf[nt][i][w] = *reinterpret_cast<const f4v*>(q + kd[i] + 4 * w);
     }
-    const int all_see = min(before + tile * PAIRS / G + 1, kv);  // positions that every row of the tile sees
+    const int all_see = min(before + t.row_of(tile * PAIRS) + 1, kv);  // positions that every row of the tile sees
 
     // ---- one pass over the range's positions -------------------------------------------------------------
     u4v kr[TILES][KW], vr[VROWS][VW];
-    bool ok[TILES][WIDE ? 1 : 4];   // whether this lane's value rows have a page
-    long koff[TILES], voff[WIDE ? TILES : VROWS];
-    bool lost = false, lost_next = false, ok_next[TILES][WIDE ? 1 : 4];
-    long koff_next[TILES], voff_next[WIDE ? TILES : VROWS];
-    auto place = [&](int c) {  // where the step's rows lie
-      lost_next = false;
+    // Where the next step's rows lie: an offset for each tile of 16 rows (wide pages, the same for the whole wave), or
+    // for each of the lane's key and value rows; and whether a page holds them, a bit each.
+    long off[WIDE ? TILES : 5 * TILES];
+    uint32_t held = 0, held_next = 0;
+    constexpr uint32_t ALL = WIDE ? (1u << TILES) - 1 : (1u << 4 * TILES) - 1;
+    int pages[WIDE ? TILES : 1];
+    auto look_up = [&](int c) {
+      if constexpr (WIDE) {
+#pragma unroll
+        for (int u = 0; u < TILES; ++u) pages[u] = a.kv.table[base + (min(c + 16 * u, j1 - 1) >> sh)];
+      }
+    };
+    auto place = [&](int c) {
+      held_next = 0;
       if constexpr (WIDE) {
 #pragma unroll
         for (int u = 0; u < TILES; ++u) {
           const int cu = c + 16 * u;
-          int page = -1;
-          if (cu < j1) page = a.kv.table[base + (cu >> sh)];
-          const bool real = static_cast<uint32_t>(page) < static_cast<uint32_t>(a.kv.n_pages);
-          ok_next[u][0] = real;
-          lost_next |= !real;
-          koff_next[u] = real ? page * a.kv.page_stride + ((static_cast<long>(kvh) << sh) + (cu & pmask)) * hd : 0;
-          voff_next[u] = koff_next[u];
+          const bool real = static_cast<uint32_t>(pages[u]) < static_cast<uint32_t>(a.kv.n_pages) && cu < j1;
+          held_next |= real ? 1u << u : 0u;
+          off[u] = real ? pages[u] * a.kv.page_stride + ((static_cast<long>(kvh) << sh) + (cu & pmask)) * hd : 0;
         }
       } else {
 #pragma unroll
@@ -133,54 +112,88 @@ __global__ __launch_bounds__(kFewWaves * kWave, HDP == 256 ? 1 : (HDP == 64 ? 3 
           long ko = 0, vo = 0;
           const int jk = c + 16 * u + m;
           if (!(jk < j1 && kv_offset<true>(a.kv, kvh, hd, base, jk, &ko, &vo))) ko = 0;
-          koff_next[u] = ko;
+          off[5 * u] = ko;
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             const int jv = c + 16 * u + 4 * g4 + r;
             ko = vo = 0;
             const bool real = jv < j1 && kv_offset<true>(a.kv, kvh, hd, base, jv, &ko, &vo);
-            ok_next[u][r] = real;
-            lost_next |= !real;
-            voff_next[4 * u + r] = real ? vo : 0;
+            held_next |= real ? 1u << (4 * u + r) : 0u;
+            off[5 * u + 1 + r] = real ? vo : 0;
           }
         }
-        lost_next = __any(lost_next);
       }
     };
     auto load_k = [&]() {
 #pragma unroll
-      for (int u = 0; u < TILES; ++u) {
-        const T* row = kp + koff[u] + (WIDE ? m * hd : 0);
+      for (int u = 0; u < TILES; ++u)
 #pragma unroll
-        for (int i = 0; i < KW; ++i) kr[u][i] = *reinterpret_cast<const u4v*>(row + kd[i]);
-      }
+        for (int i = 0; i < KW; ++i) {
+          if constexpr (WIDE) kr[u][i] = *reinterpret_cast<const u4v*>(reinterpret_cast<const char*>(kp + off[u]) + kb[i]);
+          else kr[u][i] = *reinterpret_cast<const u4v*>(kp + off[5 * u] + kd[i]);
+        }
     };
     auto load_v = [&]() {
 #pragma unroll
-      for (int j = 0; j < VROWS; ++j) {
-        const T* row = WIDE ? vp + voff[j / 4] + (4 * g4 + j % 4) * hd : vp + voff[WIDE ? 0 : j];
+      for (int j = 0; j < VROWS; ++j)
 #pragma unroll
         for (int i = 0; i < VW; ++i) {
+          const char* at;
+          if constexpr (WIDE) at = reinterpret_cast<const char*>(vp + off[j / 4] + j % 4 * hd) + vb[i];
+          else at = reinterpret_cast<const char*>(vp + off[5 * (j / 4) + 1 + j % 4] + vd[i]);
           if constexpr (!F32 && DP == 4) {
-            const u2v x = *reinterpret_cast<const u2v*>(row + vd[i]);
+            const u2v x = *reinterpret_cast<const u2v*>(at);
             vr[j][i] = u4v{x[0], x[1], 0, 0};
           } else {
-            vr[j][i] = *reinterpret_cast<const u4v*>(row + vd[i]);
+            vr[j][i] = *reinterpret_cast<const u4v*>(at);
           }
         }
-      }
     };
-    auto take_place = [&]() {
+
+    constexpr int STEP = kFewWaves * KT;
+    int c = j0 + wave * KT;
+    if (c < j1) {
+      look_up(c);
+      place(c);
+      load_k();
+      load_v();
+      look_up(c + STEP);
+    }
+    // ---- queries as operands ------------------------------------------------------------------------------
+    u4v qp[F32 ? 1 : NT][KW][NS];
+    float c2[NT];
 #pragma unroll
-      for (int u = 0; u < TILES; ++u) {
-        koff[u] = koff_next[u];
+    for (int nt = 0; nt < NT; ++nt) {
+      c2[nt] = a.c2;
 #pragma unroll
-        for (int r = 0; r < (WIDE ? 1 : 4); ++r) ok[u][r] = ok_next[u][r];
+      for (int i = 0; i < KW; ++i)
+        if (F32 ? 16 * i + 4 * g4 >= hd : 32 * i + 8 * g4 >= hd) {
+#pragma unroll
+          for (int w = 0; w < QW; ++w) qf[nt][i][w] = f4v{0, 0, 0, 0};
+        }
+      if constexpr (!F32) {
+        int e = 0;
+        if constexpr (std::is_same_v<T, _Float16>) {
+          float top = 0.0f;
+#pragma unroll
+          for (int i = 0; i < KW; ++i)
+#pragma unroll
+            for (int u = 0; u < 8; ++u) top = fmaxf(top, fabsf(qf[nt][i][u / 4][u % 4]));
+          e = query_exponent(column_max(top));
+          c2[nt] = ldexpf(c2[nt], -e);
+        }
+#pragma unroll
+        for (int i = 0; i < KW; ++i) {
+          float x[8];
+#pragma unroll
+          for (int u = 0; u < 8; ++u) {
+            x[u] = qf[nt][i][u / 4][u % 4];
+            if constexpr (std::is_same_v<T, _Float16>) x[u] = ldexpf(x[u], e);
+          }
+          split8<T>(x, qp[nt][i]);
+        }
       }
-#pragma unroll
-      for (int u = 0; u < (WIDE ? TILES : VROWS); ++u) voff[u] = voff_next[u];
-      lost = lost_next;
-    };
+    }
 
     f4v o[NT][DP];
     float sub[NT], l[NT];
@@ -191,23 +204,10 @@ __global__ __launch_bounds__(kFewWaves * kWave, HDP == 256 ? 1 : (HDP == 64 ? 3 
       sub[nt] = -INFINITY;
       l[nt] = 0.0f;
     }
-    constexpr int STEP = kFewWaves * KT;
-    int c = j0 + wave * KT;
-    if (c < j1) {
-      place(c);
-      take_place();
-      load_k();
-      load_v();
-      place(c + STEP);
-    }
     for (; c < j1; c += STEP) {
       const bool more = c + STEP < j1;
-      const bool partial = lost || c + KT > all_see;
-      bool okc[TILES][WIDE ? 1 : 4];
-#pragma unroll
-      for (int u = 0; u < TILES; ++u)
-#pragma unroll
-        for (int r = 0; r < (WIDE ? 1 : 4); ++r) okc[u][r] = ok[u][r];
+      held = held_next;
+      const bool partial = (WIDE ? held != ALL : __any(held != ALL)) || c + KT > all_see;
       f4v sc[NT][TILES];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
@@ -219,7 +219,7 @@ __global__ __launch_bounds__(kFewWaves * kWave, HDP == 256 ? 1 : (HDP == 64 ? 3 
             for (int i = 0; i < KW; ++i)
 #pragma unroll
               for (int s = 0; s < 4; ++s)
-                part[i & 1] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kr[u][i][s]), qf[nt][i][s], part[i & 1], 0, 0, 0);
+                part[i & 1] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kr[u][i][s]), qf[nt][i][0][s], part[i & 1], 0, 0, 0);
             sc[nt][u] = part[0] + part[1];
           } else {
             f4v acc = {0, 0, 0, 0};
@@ -231,27 +231,28 @@ __global__ __launch_bounds__(kFewWaves * kWave, HDP == 256 ? 1 : (HDP == 64 ? 3 
           }
         }
       if (more) {
-        take_place();
+        place(c + STEP);
         load_k();
+        look_up(c + 2 * STEP);
       }
       if (partial) {
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int u = 0; u < TILES; ++u) {
+          const int at = c + 16 * u + 4 * g4;  // the lane's first position of the tile
 #pragma unroll
-          for (int u = 0; u < TILES; ++u)
+          for (int r = 0; r < 4; ++r) {
+            const bool real = held >> (WIDE ? u : 4 * u + r) & 1;
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-              if (c + 16 * u + 4 * g4 + r >= min(seen[nt], j1) || !okc[u][WIDE ? 0 : r]) sc[nt][u][r] = -INFINITY;
-#pragma unroll
-        for (int u = 0; u < TILES; ++u)
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (c + 16 * u + 4 * g4 + r >= j1 || !okc[u][WIDE ? 0 : r]) {
+            for (int nt = 0; nt < NT; ++nt)
+              if (at + r >= (real ? min(seen[nt], j1) : 0)) sc[nt][u][r] = -INFINITY;
+            if (at + r >= (real ? j1 : 0)) {
 #pragma unroll
               for (int i = 0; i < VW; ++i) vr[4 * u + r][i] = u4v{0, 0, 0, 0};
             }
+          }
+        }
       }
-      float p[NT][8];
+      float p[NT][4 * TILES];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         float cm = -INFINITY;
@@ -282,33 +283,38 @@ __global__ __launch_bounds__(kFewWaves * kWave, HDP == 256 ? 1 : (HDP == 64 ? 3 
       }
       if constexpr (F32) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
+        for (int r = 0; r < VROWS; ++r)
 #pragma unroll
           for (int d = 0; d < DP; ++d)
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
               o[nt][d] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vr[r][d / 4][d % 4]), p[nt][r], o[nt][d], 0, 0, 0);
       } else {
-        u4v pp[NT][NS];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) split8<T>(p[nt], pp[nt]);
+        for (int gr = 0; gr < TILES / 2; ++gr) {  // 32 positions: one product
+          u4v pp[NT][NS];
 #pragma unroll
-        for (int d = 0; d < DP; ++d) {
-          u4v v;  // dim m DP + d of the lane's eight value rows
+          for (int nt = 0; nt < NT; ++nt) {
+            float x[8];
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            v[i] = __builtin_amdgcn_perm(vr[(2 * i + 1) % VROWS][d / 8][d % 8 / 2], vr[2 * i % VROWS][d / 8][d % 8 / 2],
-                                         d % 2 ? 0x07060302u : 0x05040100u);
+            for (int i = 0; i < 8; ++i) x[i] = p[nt][8 * gr + i];
+            split8<T>(x, pp[nt]);
+          }
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
+          for (int d = 0; d < DP; ++d) {
+            u4v v;  // dim m DP + d of the lane's eight value rows
 #pragma unroll
-            for (int s = NS - 1; s >= 0; --s) o[nt][d] = mfma16<T>(v, pp[nt][s], o[nt][d]);
+            for (int i = 0; i < 4; ++i)
+              v[i] = __builtin_amdgcn_perm(vr[8 * gr + 2 * i + 1][d / 8][d % 8 / 2], vr[8 * gr + 2 * i][d / 8][d % 8 / 2],
+                                           d % 2 ? 0x07060302u : 0x05040100u);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int s = NS - 1; s >= 0; --s) o[nt][d] = mfma16<T>(v, pp[nt][s], o[nt][d]);
+          }
         }
       }
-      if (more) {
-        load_v();
-        place(c + 2 * STEP);
-      }
+      if (more) load_v();
     }
 
     // ---- the waves' sums joined ------------------------------------------------------------------------
@@ -325,10 +331,16 @@ __global__ __launch_bounds__(kFewWaves * kWave, HDP == 256 ? 1 : (HDP == 64 ? 3 
     const int pairs = min(n * G - tile * PAIRS, PAIRS);
     const bool direct = ns == 1;
     auto place_of = [&](int pair, long* out_row, long* part_row) {
-      const int p = tile * PAIRS + pair, row = p / G, head = kvh * G + p - row * G;
+      const int p = tile * PAIRS + pair, row = t.row_of(p), head = kvh * G + p - row * G;
       *out_row = (first + row) * a.ldo + static_cast<long>(head) * hd;
       *part_row = (static_cast<long>(split) * a.max_rows + first + row) * a.H + head;
     };
+    if (split == 0 && t.count != nullptr) {
+      for (int p = tid; p < pairs; p += kFewWaves * kWave) {
+        const int row = t.row_of(tile * PAIRS + p);
+        t.count[static_cast<long>(first + row) * a.H + kvh * G + tile * PAIRS + p - row * G] = ns;
+      }
+    }
     bool bad = false;
     for (int idx = tid; idx < pairs * (hd / 4); idx += kFewWaves * kWave) {
       const int pair = idx / (hd / 4), d = 4 * (idx - pair * (hd / 4));
@@ -361,7 +373,7 @@ __global__ __launch_bounds__(kFewWaves * kWave, HDP == 256 ? 1 : (HDP == 64 ? 3 
       // some row sees an infinity or NaN, or has one beside what it sees: each pair again by itself
       float* qs = o_s[wave];
       for (int pair = wave; pair < pairs; pair += kFewWaves) {
-        const int p = tile * PAIRS + pair, row = p / G, head = kvh * G + p - row * G;
+        const int p = tile * PAIRS + pair, row = t.row_of(p), head = kvh * G + p - row * G;
         const float* q = a.q + (first + row) * a.ldq + static_cast<long>(head) * hd;
         for (int d = lane; d < hd; d += kWave) qs[d] = q[d];
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -388,49 +400,81 @@ __global__ __launch_bounds__(kFewWaves * kWave, HDP == 256 ? 1 : (HDP == 64 ? 3 
   }
 }
 
-// Each (row, head) of a request whose positions were split: its ranges' sums added, a wave each.
+// Each (row, head) whose positions were split: its ranges' sums added, by one wave.  A lane takes 4 dims of every
+// (64 / (hd / 4))th range.  The lengths are not read: the first range's workgroup left their number beside its
+// sums, and the loads of the first ranges do not wait for it (what they read beyond it is not used).
+constexpr int kJoinFirst = 4;
+
+template <int LANES>  // lanes to a row: 16, 32 or 64
 __global__ __launch_bounds__(256) void attention_join_kernel(AttnTask t) {
+  constexpr int GROUPS = kWave / LANES;
   const RowsArgs& a = t.r;
   const int wave = threadIdx.x / kWave, lane = threadIdx.x & (kWave - 1);
-  const int row = blockIdx.x, h = blockIdx.y * 4 + wave;
-  if (row >= min(a.row_start[a.n_seqs], a.max_rows) || h >= a.H) return;
-  const int req = request_of(a.row_start, a.n_seqs, row);
-  const int kv = static_cast<int>(min(static_cast<long>(a.kv_len[req]), a.kv.table_ld << a.kv.page_shift));
-  const long pairs = static_cast<long>(a.row_start[req + 1] - a.row_start[req]) * (a.H / a.KV);
-  const int ns = splits_of(kv, pairs <= t.few_most ? t.few_split : t.tile_split);
-  if (ns == 1) return;
-  const long step = static_cast<long>(a.max_rows) * a.H, at = static_cast<long>(row) * a.H + h;
-  float top = -INFINITY;
-  for (int s = lane; s < ns; s += kWave) top = fmaxf(top, t.stat[s * step + at][0]);
+  const long at = static_cast<long>(blockIdx.x) * 4 + wave, step = static_cast<long>(a.max_rows) * a.H;
+  const int group = lane / LANES, d = 4 * (lane % LANES), most = max(t.few_split.splits, t.tile_split.splits);
+  const long rows = min(a.row_start[a.n_seqs], a.max_rows);
+  if (at >= step) return;
+  const bool in = d < a.hd;
+  const float* part = t.part + at * a.hd + (in ? d : 0);
+  const int ns = t.count[at];
+  f4v first[kJoinFirst];
+#pragma unroll
+  for (int i = 0; i < kJoinFirst; ++i) first[i] = *reinterpret_cast<const f4v*>(part + min(group + i * GROUPS, most - 1) * step * a.hd);
+  f2v st = t.stat[min(lane, most - 1) * step + at];
+  if (at >= rows * a.H || ns <= 1) return;
+  float top = lane < ns ? st[0] : -INFINITY;
+  for (int s = lane + kWave; s < ns; s += kWave) top = fmaxf(top, t.stat[s * step + at][0]);
   top = wave_max_dpp(top);
-  float l = 0.0f, o[4] = {0, 0, 0, 0};
-  for (int s = 0; s < ns; ++s) {
-    const f2v st = t.stat[s * step + at];
-    const float f = st[0] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(st[0] - top);
-    l = fmaf(st[1], f, l);
-    const float* p = t.part + (s * step + at) * a.hd;
+  float l = 0.0f;
+  f4v o = {0, 0, 0, 0};
+  for (int s0 = 0; s0 < ns; s0 += kWave) {
+    if (s0 > 0) st = t.stat[min(s0 + lane, ns - 1) * step + at];
+    const float w = s0 + lane < ns && st[0] != -INFINITY ? __builtin_amdgcn_exp2f(st[0] - top) : 0.0f;
+    if (s0 + lane < ns) l = fmaf(st[1], w, l);
+    const int end = min(ns - s0, kWave);
+    int s = group;
+    if (s0 == 0) {
 #pragma unroll
-    for (int u = 0; u < 4; ++u)
-      if (lane + 64 * u < a.hd) o[u] = fmaf(p[lane + 64 * u], f, o[u]);
+      for (int i = 0; i < kJoinFirst; ++i, s += GROUPS) {
+        const float f = __shfl(w, s & 63, kWave);
+        if (s < end) {
+#pragma unroll
+          for (int u = 0; u < 4; ++u) o[u] = fmaf(first[i][u], f, o[u]);
+        }
+      }
+    }
+    for (; s - group < end; s += GROUPS) {  // the same trip count for every group
+      const float f = __shfl(w, s & 63, kWave);
+      if (s < end) {
+        const f4v x = *reinterpret_cast<const f4v*>(part + (s0 + s) * step * a.hd);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) o[u] = fmaf(x[u], f, o[u]);
+      }
+    }
   }
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  float* out = a.out + row * a.ldo + static_cast<long>(h) * a.hd;
+  l = wave_sum(l);
 #pragma unroll
-  for (int u = 0; u < 4; ++u)
-    if (lane + 64 * u < a.hd) out[lane + 64 * u] = o[u] * inv;
+  for (int off = LANES; off < kWave; off <<= 1) {
+#pragma unroll
+    for (int u = 0; u < 4; ++u) o[u] += __shfl_xor(o[u], off, kWave);
+  }
+  if (group != 0 || !in) return;
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  const long row = at / a.H;
+  *reinterpret_cast<f4v*>(a.out + row * a.ldo + (at - row * a.H) * a.hd + d) = o * inv;
 }
 
 template <class T, int HDP, int NT>
 void run_few(const AttnTask& t, hipStream_t s) {
-  const dim3 grid(t.r.n_seqs * t.r.KV * t.tiles, t.few_split.splits);
+  const dim3 grid(t.r.n_seqs, t.r.KV, t.few_split.splits * t.tiles);
   if (t.r.kv.page_shift >= 4) attention_few_kernel<T, HDP, NT, true><<<grid, kFewWaves * kWave, 0, s>>>(t);
   else attention_few_kernel<T, HDP, NT, false><<<grid, kFewWaves * kWave, 0, s>>>(t);
 }
 
 template <class T>
 void run_few_of(const AttnTask& t, hipStream_t s) {
-  if (t.r.hd <= 64) run_few<T, 64, 1>(t, s);
-  else if (t.r.hd <= 128) run_few<T, 128, 1>(t, s);
+  if (t.r.hd <= 64) t.few_wide ? run_few<T, 64, 2>(t, s) : run_few<T, 64, 1>(t, s);
+  else if (t.r.hd <= 128) t.few_wide ? run_few<T, 128, 2>(t, s) : run_few<T, 128, 1>(t, s);
   else run_few<T, 256, 1>(t, s);
 }
 
@@ -445,7 +489,10 @@ int launch_attention_few(const AttnTask& t, int qtype, hipStream_t s) {
 }
 
 int launch_attention_join(const AttnTask& t, hipStream_t s) {
-  attention_join_kernel<<<dim3(t.r.max_rows, (t.r.H + 3) / 4), 256, 0, s>>>(t);
+  const unsigned blocks = static_cast<unsigned>((static_cast<long>(t.r.max_rows) * t.r.H + 3) / 4);
+  if (t.r.hd <= 64) attention_join_kernel<16><<<blocks, 256, 0, s>>>(t);
+  else if (t.r.hd <= 128) attention_join_kernel<32><<<blocks, 256, 0, s>>>(t);
+  else attention_join_kernel<64><<<blocks, 256, 0, s>>>(t);
   EFH_HIP(hipGetLastError());
   return EF_HIP_OK;
 }

@@ -110,7 +110,7 @@ __global__ __launch_bounds__(kTileThreads, HDP == 64 && sizeof(T) == 2 ? 3 : HDP
   const RowsArgs& a = t.r;
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid & (kWave - 1);
   const int col = lane & 31, h = lane >> 5;
-  const int G = a.H / a.KV, hd = a.hd;
+  const int G = t.group, hd = a.hd;
   // the last places first: a request's last rows see the most positions
   const int kvh = blockIdx.x % a.KV;
   const long place = static_cast<long>(gridDim.x / a.KV) - 1 - blockIdx.x / a.KV;
@@ -137,14 +137,14 @@ __global__ __launch_bounds__(kTileThreads, HDP == 64 && sizeof(T) == 2 ? 3 : HDP
   const int pairs = n * G;  // above few_most, and below 2^31 (checked on the host)
   const int pair0 = static_cast<int>(tile) * kTilePairs, pair = pair0 + 32 * wave + col;
   const bool active = pair < pairs;
-  const int row = active ? pair / G : 0, head = kvh * G + (active ? pair - row * G : 0);
+  const int row = active ? t.row_of(pair) : 0, head = kvh * G + (active ? pair - row * G : 0);
   const int seen = active ? min(before + row + 1, kv) : 0;
   const int tile_last = min(pair0 + kTilePairs, pairs) - 1;
   // positions: those of the split that the tile's last row sees
   const int j0 = split * t.tile_split.span;
-  const int j1 = min(split == t.tile_split.splits - 1 ? kv : min(kv, j0 + t.tile_split.span), min(before + tile_last / G + 1, kv));
+  const int j1 = min(split == t.tile_split.splits - 1 ? kv : min(kv, j0 + t.tile_split.span), min(before + t.row_of(tile_last) + 1, kv));
   const bool busy = pair0 + 32 * wave < pairs;  // a wave without a pair only stages
-  const int all_see = min(before + (pair0 + 32 * wave) / G + 1, kv);  // positions that every row of the wave sees
+  const int all_see = min(before + t.row_of(pair0 + 32 * wave) + 1, kv);  // positions that every row of the wave sees
 
   u4v qp[KK][NS];
   float c2 = a.c2;
@@ -386,6 +386,7 @@ __global__ __launch_bounds__(kTileThreads, HDP == 64 && sizeof(T) == 2 ? 3 : HDP
         if (dim < hd) *reinterpret_cast<f4v*>(dst + dim) = f4v{o[d][4 * q], o[d][4 * q + 1], o[d][4 * q + 2], o[d][4 * q + 3]} * inv;
       }
     if (!direct && h == 0) t.stat[part_row] = f2v{sub, l};
+    if (split == 0 && h == 0 && t.count != nullptr) t.count[static_cast<long>(first + row) * a.H + head] = ns;
   }
   uint64_t todo = __ballot(bad && active);
   todo = (todo | todo >> 32) & 0xFFFFFFFFull;

@@ -24,10 +24,19 @@ int check_rows(const RowsArgs& a, size_t heads, size_t KV, size_t n_seqs, size_t
   return EF_HIP_OK;
 }
 
+AttnTask task_of(const RowsArgs& a) {
+  AttnTask t{};
+  t.r = a;
+  t.few_split = t.tile_split = Split{1, 0x40000000};
+  t.group = a.H / a.KV;
+  t.magic = static_cast<uint32_t>(((uint64_t(1) << 32) + t.group - 1) / t.group);
+  return t;
+}
+
 // How a call of paged attention runs: the few-rows kernel for requests of up to few_most (row, head) pairs of a KV
 // head, the tiles kernel for those above, either alone where the bounds leave no request to the other.
 struct PagedPlan {
-  bool few = false, tiles = false;
+  bool few = false, tiles = false, few_wide = false;
   int few_most = 0, few_tiles = 1;
   Split few_split{1, 0x40000000}, tile_split{1, 0x40000000};
   size_t bytes = 0;  // workspace
@@ -53,14 +62,16 @@ PagedPlan plan_paged(size_t H, size_t KV, size_t hd, size_t n_seqs, size_t max_r
   const size_t few_pairs = p.tiles ? std::max<size_t>(kFewPairs, G) : pairs;
   if (p.few) {
     p.few_most = p.tiles ? static_cast<int>(few_pairs) : 0x7FFFFFFF;
-    p.few_tiles = static_cast<int>((few_pairs + kFewPairs - 1) / kFewPairs);
+    p.few_wide = few_pairs > kFewPairs && hd <= 128;
+    const size_t per = p.few_wide ? 2 * kFewPairs : kFewPairs;
+    p.few_tiles = static_cast<int>((few_pairs + per - 1) / per);
     p.few_split = split_over(n_seqs * KV * p.few_tiles, kFewWorkgroups, longest, kFewSpanLeast, kFewSpanMost, kFewStep);
   }
   if (p.tiles)
     p.tile_split = split_over((max_rows * G + kTilePairs - 1) / kTilePairs * KV + 1, kTileWorkgroups, longest, kTileSpanLeast,
                               0x40000000, kTileStep);
   const size_t splits = std::max(p.few_split.splits, p.tile_split.splits);
-  if (splits > 1) p.bytes = max_rows * H * splits * (hd + 2) * sizeof(float);
+  if (splits > 1) p.bytes = max_rows * H * (splits * (hd + 2) + 1) * sizeof(float);
   return p;
 }
 
@@ -107,18 +118,19 @@ int ef_hip_paged_attention(const float* q, size_t ldq, float* out, size_t ldo, s
   const PagedPlan p = plan_paged(heads, pool->KV, pool->hd, b.n_seqs, b.max_rows, b.max_new, b.max_kv);
   EFH_CHECK(p.bytes == 0 || (ws != nullptr && ws_bytes >= p.bytes && aligned16(ws)),
             "paged_attention: the workspace must have ef_hip_paged_attention_workspace_bytes bytes, at a multiple of 16");
-  EFH_CHECK(b.n_seqs * pool->KV <= size_t(0x7FFFFFFF) / p.few_tiles, "paged_attention: too many requests and heads");
+  EFH_CHECK(static_cast<size_t>(p.few_tiles) * p.few_split.splits <= 65535, "paged_attention: too many heads to a KV head");
   EFH_RC(require_ready());
   if (b.max_rows == 0) return EF_HIP_OK;
-  AttnTask t{};
-  t.r = a;
+  AttnTask t = task_of(a);
   t.few_split = p.few_split;
   t.tile_split = p.tile_split;
   t.tiles = p.few_tiles;
+  t.few_wide = p.few_wide;
   t.few_most = p.few_most;
   const size_t splits = std::max(p.few_split.splits, p.tile_split.splits);
   t.part = static_cast<float*>(ws);
   t.stat = reinterpret_cast<f2v*>(t.part + b.max_rows * heads * splits * pool->hd);
+  t.count = splits > 1 ? reinterpret_cast<int*>(t.stat + b.max_rows * heads * splits) : nullptr;
   hipStream_t s = pick(stream);
   if (p.tiles) EFH_RC(launch_attention_tiles(t, pool->qtype, true, s));
   if (p.few) EFH_RC(launch_attention_few(t, pool->qtype, s));
@@ -159,9 +171,7 @@ int ef_hip_packed_attention(const float* q, size_t ldq, const void* k, size_t ld
   (void)ws, (void)ws_bytes;
   EFH_RC(require_ready());
   if (max_rows == 0) return EF_HIP_OK;
-  AttnTask t{};
-  t.r = a;
-  t.tile_split = Split{1, 0x40000000};
+  const AttnTask t = task_of(a);
   return launch_attention_tiles(t, qtype, false, pick(stream));
 }
 
