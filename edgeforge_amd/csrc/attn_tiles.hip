@@ -278,22 +278,24 @@ __global__ __launch_bounds__(kTileThreads, HDP == 64 && sizeof(T) == 2 ? 3 : HDP
 
     f16v sc[SUB];
 #pragma unroll
-    for (int s = 0; s < SUB; ++s) {
+    for (int s = 0; s < SUB; ++s)
 #pragma unroll
       for (int i = 0; i < 16; ++i) sc[s][i] = 0.0f;
-      u4v kf[KK][PLANES];
 #pragma unroll
-      for (int k = 0; k < KK; ++k)
+    for (int k = 0; k < KK; ++k) {
+      u4v kf[SUB][PLANES];
+#pragma unroll
+      for (int s = 0; s < SUB; ++s)
 #pragma unroll
         for (int p = 0; p < PLANES; ++p)
-          kf[k][p] = *reinterpret_cast<const u4v*>(kt + p * PLANE + 32 * s * HDP + 8 * k_place<CHUNKS>(2 * k + h, col));
+          kf[s][p] = *reinterpret_cast<const u4v*>(kt + p * PLANE + 32 * s * HDP + 8 * k_place<CHUNKS>(2 * k + h, col));
 #pragma unroll
-      for (int k = 0; k < KK; ++k)
+      for (int sum = NS - 1; sum >= 0; --sum)  // the small products first; the sums in turn, as each waits for itself
 #pragma unroll
-        for (int sum = NS - 1; sum >= 0; --sum)  // the small products first
+        for (int p = 0; p < PLANES; ++p)
 #pragma unroll
-          for (int p = 0; p < PLANES; ++p)
-            if (sum - p >= 0) sc[s] = mfma32<T>(kf[k][p], qp[k][sum - p], sc[s]);
+          for (int s = 0; s < SUB; ++s)
+            if (sum - p >= 0) sc[s] = mfma32<T>(kf[s][p], qp[k][sum - p], sc[s]);
     }
     if (c + BN > all_see) {
 #pragma unroll
@@ -343,22 +345,27 @@ __global__ __launch_bounds__(kTileThreads, HDP == 64 && sizeof(T) == 2 ? 3 : HDP
         }
         u4v pp[NS];
         split8<T>(p, pp);
+        constexpr int TURN = DT < 4 ? DT : 4;  // sums taken in turn
 #pragma unroll
-        for (int d = 0; d < DT; ++d) {
-          u4v vf[PLANES];
+        for (int d0 = 0; d0 < DT; d0 += TURN) {
+          u4v vf[TURN][PLANES];
 #pragma unroll
-          for (int pl = 0; pl < PLANES; ++pl) {
-            uint16_t* at = const_cast<uint16_t*>(vt) + pl * PLANE + (32 * s + 16 * half) * HDP + 8 * v_place<CHUNKS>(4 * d + vchunk, vq);
-            const s4v lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4v)at);
-            const s4v hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4v)(at + 8 * HDP));
-            const u2v lw = __builtin_bit_cast(u2v, lo), hw = __builtin_bit_cast(u2v, hi);
-            vf[pl] = u4v{lw[0], lw[1], hw[0], hw[1]};
-          }
+          for (int d = 0; d < TURN; ++d)
+#pragma unroll
+            for (int pl = 0; pl < PLANES; ++pl) {
+              uint16_t* at = const_cast<uint16_t*>(vt) + pl * PLANE + (32 * s + 16 * half) * HDP + 8 * v_place<CHUNKS>(4 * (d0 + d) + vchunk, vq);
+              const s4v lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4v)at);
+              const s4v hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4v)(at + 8 * HDP));
+              const u2v lw = __builtin_bit_cast(u2v, lo), hw = __builtin_bit_cast(u2v, hi);
+              vf[d][pl] = u4v{lw[0], lw[1], hw[0], hw[1]};
+            }
 #pragma unroll
           for (int ps = NS - 1; ps >= 0; --ps)
 #pragma unroll
             for (int pl = 0; pl < PLANES; ++pl)
-              if (ps - pl >= 0) o[d] = mfma32<T>(vf[pl], pp[ps - pl], o[d]);
+#pragma unroll
+              for (int d = 0; d < TURN; ++d)
+                if (ps - pl >= 0) o[d0 + d] = mfma32<T>(vf[d][pl], pp[ps - pl], o[d0 + d]);
         }
       }
     }

@@ -42,20 +42,24 @@ struct PagedPlan {
   size_t bytes = 0;  // workspace
 };
 constexpr int kFewPairs = 16, kFewAlone = 64;
-constexpr int kFewStep = 128, kFewSpanLeast = 256, kFewSpanMost = 4096, kFewWorkgroups = 1024;
-constexpr int kTileStep = 64, kTileSpanLeast = 512, kTileWorkgroups = 512;
+constexpr int kFewStep = 128;
+constexpr int kTileStep = 64, kTileSpanLeast = 256;
 
-// Ranges of positions so that `wgs` workgroups per range make about `want`, none shorter than `least`.
-Split split_over(size_t wgs, size_t want, size_t longest, size_t least, size_t most, size_t step) {
-  const size_t ranges = (want + wgs - 1) / wgs;
-  size_t span = std::min(std::max((longest + ranges - 1) / ranges, least), most);
+// Ranges of positions: as many as make `wgs` workgroups per range about `want` in all, but none shorter than `least`.
+Split split_over(size_t wgs, size_t want, size_t longest, size_t least, size_t step) {
+  const size_t ranges = std::max<size_t>(want / wgs, 1);
+  size_t span = std::max((longest + ranges - 1) / ranges, least);
   span = std::max(span, (longest + 1023) / 1024);
   span = (span + step - 1) / step * step;
   return Split{static_cast<int>((longest + span - 1) / span), static_cast<int>(span)};
 }
 
-PagedPlan plan_paged(size_t H, size_t KV, size_t hd, size_t n_seqs, size_t max_rows, size_t max_new, size_t max_kv) {
+// Positions are split so that the workgroups fill the GPU once (as many as its CUs hold at the kernels' registers): one
+// more than fits costs a second round.  12 x 32k BF16: 5 ranges (480 workgroups of 512) 215 us, 8 (768) 271, 10 (960)
+// 237; 64 requests of 2047 FP16: 3 ranges (768 of 768) 26.8 us, 4 (1024) 32.
+PagedPlan plan_paged(size_t H, size_t KV, size_t hd, int qtype, size_t n_seqs, size_t max_rows, size_t max_new, size_t max_kv) {
   PagedPlan p;
+  const size_t cus = ctx().cu_count > 0 ? ctx().cu_count : 256;
   const size_t G = H / KV, pairs = std::max<size_t>(max_new, 1) * G, longest = std::max<size_t>(max_kv, 1);
   p.few = pairs <= kFewAlone || n_seqs > 1;
   p.tiles = pairs > kFewAlone;
@@ -65,11 +69,11 @@ PagedPlan plan_paged(size_t H, size_t KV, size_t hd, size_t n_seqs, size_t max_r
     p.few_wide = few_pairs > kFewPairs && hd <= 128;
     const size_t per = p.few_wide ? 2 * kFewPairs : kFewPairs;
     p.few_tiles = static_cast<int>((few_pairs + per - 1) / per);
-    p.few_split = split_over(n_seqs * KV * p.few_tiles, kFewWorkgroups, longest, kFewSpanLeast, kFewSpanMost, kFewStep);
+    p.few_split = split_over(n_seqs * KV * p.few_tiles, cus * (hd <= 64 ? 3 : hd <= 128 ? 2 : 1), longest, kFewStep, kFewStep);
   }
   if (p.tiles)
-    p.tile_split = split_over((max_rows * G + kTilePairs - 1) / kTilePairs * KV + 1, kTileWorkgroups, longest, kTileSpanLeast,
-                              0x40000000, kTileStep);
+    p.tile_split = split_over(std::max<size_t>((max_rows * G + kTilePairs - 1) / kTilePairs * KV, 1),
+                              cus * (hd <= 64 && qtype != EF_QTYPE_F32 ? 3 : hd <= 128 ? 2 : 1), longest, kTileSpanLeast, kTileStep);
   const size_t splits = std::max(p.few_split.splits, p.tile_split.splits);
   if (splits > 1) p.bytes = max_rows * H * (splits * (hd + 2) + 1) * sizeof(float);
   return p;
@@ -87,7 +91,7 @@ size_t ef_hip_paged_attention_workspace_bytes(size_t heads, const ef_hip_page_po
   if (check_page_pool(pool, "paged_attention") != EF_HIP_OK || heads < 1 || heads > 65535 || heads % pool->KV != 0 ||
       n_seqs < 1 || max_rows > (size_t(1) << 30) || max_kv > 0x7FFFFFFF)
     return 0;
-  return plan_paged(heads, pool->KV, pool->hd, n_seqs, max_rows, max_new, max_kv).bytes;
+  return plan_paged(heads, pool->KV, pool->hd, pool->qtype, n_seqs, max_rows, max_new, max_kv).bytes;
 }
 
 int ef_hip_paged_attention(const float* q, size_t ldq, float* out, size_t ldo, size_t heads, const ef_hip_page_pool* pool,
@@ -115,7 +119,7 @@ int ef_hip_paged_attention(const float* q, size_t ldq, float* out, size_t ldo, s
   a.kv = KvSource{pool->k_dev, pool->v_dev, 0, 0, b.table_dev, static_cast<long>(b.table_ld),
                   static_cast<long>(pool_stride(*pool)), log2_of(pool->page_size), static_cast<int>(pool->n_pages)};
   EFH_CHECK(b.max_kv <= 0x7FFFFFFF, "paged_attention: max_kv too large");
-  const PagedPlan p = plan_paged(heads, pool->KV, pool->hd, b.n_seqs, b.max_rows, b.max_new, b.max_kv);
+  const PagedPlan p = plan_paged(heads, pool->KV, pool->hd, pool->qtype, b.n_seqs, b.max_rows, b.max_new, b.max_kv);
   EFH_CHECK(p.bytes == 0 || (ws != nullptr && ws_bytes >= p.bytes && aligned16(ws)),
             "paged_attention: the workspace must have ef_hip_paged_attention_workspace_bytes bytes, at a multiple of 16");
   EFH_CHECK(static_cast<size_t>(p.few_tiles) * p.few_split.splits <= 65535, "paged_attention: too many heads to a KV head");
