@@ -226,6 +226,13 @@ struct AttnTask {
 // (row, head) pairs of a KV head in a workgroup of the tiles kernel
 constexpr int kTilePairs = 128;
 
+// Packed FP32 and BF16 rows prepared as FP16 tiles of `rows` rows and `bytes` bytes; the workspace holds KV tiles of
+// each of the places (ceil(max_rows / rows) + n_seqs of them), then 8 bytes for each.
+struct PreparedShape {
+  size_t rows, bytes;
+};
+PreparedShape prepared_shape(size_t hd, int qtype);
+int launch_attention_prepared(const AttnTask& t, int qtype, void* ws, size_t places, hipStream_t s);
 int launch_attention_tiles(const AttnTask& t, int qtype, bool paged, hipStream_t s);
 int launch_attention_join(const AttnTask& t, hipStream_t s);
 int launch_attention_few(const AttnTask& t, int qtype, hipStream_t s);

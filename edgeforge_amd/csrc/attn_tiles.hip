@@ -59,15 +59,22 @@ __device__ __forceinline__ int request_of_place(const RowsArgs& a, long x) {
   return __builtin_amdgcn_readfirstlane(lo);
 }
 
-template <class T, int HDP>
+// Where a tile's keys and values come from.
+enum Source {
+  kPages,     // a request's pages, in their own type
+  kRows,      // packed rows, in their own type
+  kPrepared,  // packed FP32 or BF16 rows brought to FP16 by attention_prepare_kernel
+};
+
+template <class T, int HDP, int SRC>
 struct TileShape {
-  static constexpr bool F32 = sizeof(T) == 4;
+  static constexpr bool F32 = sizeof(T) == 4, PREPARED = SRC == kPrepared;
   static constexpr int BN = HDP == 256 || (F32 && HDP >= 128) ? 32 : 64;  // positions of a tile
-  static constexpr int PLANES = F32 ? 3 : 1;                              // 16-bit planes of a key or value
+  static constexpr int PLANES = !F32 ? 1 : PREPARED ? 2 : 3;              // 16-bit planes of a key or value
   static constexpr int CHUNKS = HDP / 8;                                  // 16-byte chunks of a row
   static constexpr int PLANE = BN * HDP;                                  // 16-bit values of a plane
-  static constexpr int BUFFERS = F32 ? 1 : 2;
-  static constexpr int UNITS = PLANE / 8 / kTileThreads;                  // chunks that a thread brings of keys, and of values
+  static constexpr int BUFFERS = F32 && !PREPARED ? 1 : 2;
+  static constexpr int UNITS = PLANE / 8 / kTileThreads;                  // chunks that a thread brings of a plane
 };
 
 // Rows lie in LDS without padding (a DMA instruction writes 1 KB in one piece), their 16-byte chunks in another order in
@@ -95,13 +102,125 @@ __device__ __forceinline__ void tile_barrier() {
   asm volatile("" ::: "memory");
 }
 
-template <class T, int HDP, bool PAGED>
-__global__ __launch_bounds__(kTileThreads, HDP == 64 && sizeof(T) == 2 ? 3 : HDP <= 128 ? 2 : 1) void attention_tiles_kernel(AttnTask t) {
-  using Sh = TileShape<T, HDP>;
-  constexpr bool F32 = Sh::F32;
+// ---- packed FP32 and BF16 rows as FP16 ---------------------------------------------------------------------
+// A tile of BN rows of one KV head times a power of two that brings its largest value to 2^7 .. 2^15 (its exponent a
+// multiple of 8, so that neighbouring tiles mostly share it): FP32 as two planes, the rounded half and what it left,
+// BF16 as one.  A half of a value x below 2^-14 is off by up to 2^-25: below 2^-24 of its row's largest value as long as
+// that is at least 1/2.  Tiles with a row that is smaller (and not zero), or with infinities or NaN, are marked; the
+// attention kernel takes them from the rows themselves.  Three products (high high, high low, low high) then do
+// what the three-part BF16 split needs six for, and BF16 keys and values two of three.  The tile is written
+// as the kernel's LDS holds it: planes of K, planes of V.
+// Read and written once, in one pass: bound by memory (6001 rows of 4 heads of 64: 12 + 12 MB).
+constexpr int kNoTile = INT32_MIN, kAnyScale = INT32_MAX;
+
+struct PrepareArgs {
+  KvSource kv;
+  const int32_t* row_start;
+  int n_seqs, max_rows, hd, places;
+  uint16_t* blocks;  // [KV][places][2][PLANES][BN][HDP]
+  int2* info;        // [KV][places]: exponents of K and V (kNoTile: marked; kAnyScale: all zero)
+};
+
+// Request r's tiles have the places floor(start[r] / BN) + r on, as the workgroups' places above.
+template <int BN>
+__device__ __forceinline__ long prepared_place(const int32_t* row_start, int r) { return row_start[r] / BN + r; }
+
+template <class T, int HDP>
+__global__ __launch_bounds__(kTileThreads) void attention_prepare_kernel(PrepareArgs a) {
+  using Sh = TileShape<T, HDP, kPrepared>;
+  constexpr int BN = Sh::BN, CHUNKS = Sh::CHUNKS, UNITS = Sh::UNITS, PLANES = Sh::PLANES, PLANE = Sh::PLANE, ROWS = kTileThreads / CHUNKS;
+  __shared__ uint32_t most_s[2], least_s[2];
+  const int tid = threadIdx.x, kvh = blockIdx.y, chunk = tid % CHUNKS, my_row = tid / CHUNKS;
+  const long place = blockIdx.x;
+  int lo = 0;
+  for (int len = a.n_seqs; len > 1;) {  // request_of_place with this kernel's tiles
+    const int step = (len + kWave - 1) / kWave, i = (tid & (kWave - 1)) * step;
+    const uint64_t below = __ballot(i < len && prepared_place<BN>(a.row_start, lo + i) <= place);
+    const int last = max(__popcll(below) - 1, 0) * step;
+    lo += last;
+    len = min(step, len - last);
+  }
+  const int req = __builtin_amdgcn_readfirstlane(lo), first = a.row_start[req];
+  const int n = min(a.row_start[req + 1], a.max_rows) - first;
+  const long c = (place - prepared_place<BN>(a.row_start, req)) * BN;
+  if (n <= 0 || c >= n) return;
+  if (tid < 2) {
+    most_s[tid] = 0;
+    least_s[tid] = 0xFFFFFFFFu;
+  }
+  float x[2][UNITS][8];
+#pragma unroll
+  for (int kv = 0; kv < 2; ++kv)
+#pragma unroll
+    for (int u = 0; u < UNITS; ++u) {
+      const int r = my_row + u * ROWS;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[kv][u][i] = 0.0f;
+      if (c + r < n && 8 * chunk < a.hd)
+        load8(static_cast<const T*>(kv ? a.kv.v : a.kv.k) + (first + c + r) * (kv ? a.kv.ldv : a.kv.ldk) + static_cast<long>(kvh) * a.hd + 8 * chunk, x[kv][u]);
+    }
+  __syncthreads();
+#pragma unroll
+  for (int kv = 0; kv < 2; ++kv) {
+    uint32_t most = 0, least = 0xFFFFFFFFu;
+#pragma unroll
+    for (int u = 0; u < UNITS; ++u) {
+      uint32_t top = 0;  // the row's largest magnitude, as bits (infinities and NaN are the largest)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[kv][u][i]) & 0x7FFFFFFFu);
+#pragma unroll
+      for (int o = 1; o < CHUNKS; o <<= 1) top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), o, kWave)));
+      most = max(most, top);
+      if (top) least = min(least, top);
+    }
+#pragma unroll
+    for (int o = CHUNKS; o < kWave; o <<= 1) {
+      most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), o, kWave)));
+      least = min(least, static_cast<uint32_t>(__shfl_xor(static_cast<int>(least), o, kWave)));
+    }
+    if ((tid & (kWave - 1)) == 0) {
+      atomicMax(&most_s[kv], most);
+      atomicMin(&least_s[kv], least);
+    }
+  }
+  __syncthreads();
+  int e[2];
+  bool marked = false;
+#pragma unroll
+  for (int kv = 0; kv < 2; ++kv) {
+    const uint32_t most = most_s[kv], least = least_s[kv];
+    e[kv] = most == 0 ? kAnyScale : ((14 + 127 - static_cast<int>(most >> 23)) & ~7);
+    marked = marked || most >= 0x7F800000u || (most != 0 && static_cast<int>(least >> 23) - 127 + e[kv] < -1);
+  }
+  const long at = kvh * static_cast<long>(a.places) + place;
+  if (tid == 0) a.info[at] = marked ? int2{kNoTile, kNoTile} : int2{e[0], e[1]};
+  if (marked) return;
+  uint16_t* block = a.blocks + at * (2 * PLANES * PLANE);
+#pragma unroll
+  for (int kv = 0; kv < 2; ++kv) {
+    const int scale = e[kv] == kAnyScale ? 0 : e[kv];
+#pragma unroll
+    for (int u = 0; u < UNITS; ++u) {
+      const int r = my_row + u * ROWS;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[kv][u][i] = ldexpf(x[kv][u][i], scale);
+      u4v part[2];
+      split8<_Float16>(x[kv][u], part);
+      uint16_t* dst = block + kv * PLANES * PLANE + r * HDP + 8 * (kv ? v_place<CHUNKS>(chunk, r) : k_place<CHUNKS>(chunk, r));
+#pragma unroll
+      for (int p = 0; p < PLANES; ++p) *reinterpret_cast<u4v*>(dst + p * PLANE) = part[p];
+    }
+  }
+}
+
+template <class T, int HDP, int SRC>
+__global__ __launch_bounds__(kTileThreads, HDP == 64 && sizeof(T) == 2 ? 3 : HDP <= 128 ? 2 : 1) void attention_tiles_kernel(AttnTask t, PrepareArgs pre) {
+  using Sh = TileShape<T, HDP, SRC>;
+  using C = std::conditional_t<SRC == kPrepared, _Float16, T>;  // what the products are in
+  constexpr bool PAGED = SRC == kPages, PREPARED = SRC == kPrepared, F32 = Sh::F32 && !PREPARED;
   constexpr int BN = Sh::BN, SUB = BN / 32, PLANES = Sh::PLANES, CHUNKS = Sh::CHUNKS, PLANE = Sh::PLANE, UNITS = Sh::UNITS;
-  constexpr int BUFFERS = Sh::BUFFERS, KK = HDP / 16, DT = HDP / 32, NS = Parts<T>::N;
-  constexpr float OFFSET = Parts<T>::kSubOffset;
+  constexpr int BUFFERS = Sh::BUFFERS, KK = HDP / 16, DT = HDP / 32, NS = Parts<C>::N;
+  constexpr float OFFSET = Parts<C>::kSubOffset;
   __shared__ __attribute__((aligned(1024))) uint16_t ks[BUFFERS][PLANES * PLANE];
   __shared__ __attribute__((aligned(1024))) uint16_t vs[BUFFERS][PLANES * PLANE];
   __shared__ uint32_t ok_s[2][BN / 4];  // a byte per position: whether a page holds it
@@ -148,11 +267,11 @@ __global__ __launch_bounds__(kTileThreads, HDP == 64 && sizeof(T) == 2 ? 3 : HDP
 
   u4v qp[KK][NS];
   float c2 = a.c2;
+  int e = 0;
   {
     const float* q = a.q + static_cast<long>(first + row) * a.ldq + static_cast<long>(head) * hd;
     float top = 0.0f;
-    int e = 0;
-    if constexpr (std::is_same_v<T, _Float16>) {
+    if constexpr (std::is_same_v<C, _Float16>) {
 #pragma unroll
       for (int k = 0; k < KK; ++k) {
         float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
@@ -167,11 +286,11 @@ __global__ __launch_bounds__(kTileThreads, HDP == 64 && sizeof(T) == 2 ? 3 : HDP
     for (int k = 0; k < KK; ++k) {
       float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
       if (16 * k + 8 * h < hd) load8(q + 16 * k + 8 * h, x);
-      if constexpr (std::is_same_v<T, _Float16>) {
+      if constexpr (std::is_same_v<C, _Float16>) {
 #pragma unroll
         for (int u = 0; u < 8; ++u) x[u] = ldexpf(x[u], e);
       }
-      split8<T>(x, qp[k]);
+      split8<C>(x, qp[k]);
     }
   }
 
@@ -195,7 +314,19 @@ __global__ __launch_bounds__(kTileThreads, HDP == 64 && sizeof(T) == 2 ? 3 : HDP
   u4v kr[F32 ? UNITS : 1][WORDS], vr[F32 ? UNITS : 1][WORDS];
   const uint32_t k_lds = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) void*)ks)) + 1024 * wave;
   const uint32_t v_lds = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) void*)vs)) + 1024 * wave;
+  int2 info = {0, 0};  // of the tile brought last
   auto bring = [&](int c, int buf, int ok_buf) {
+    if constexpr (PREPARED) {
+      const long at = kvh * static_cast<long>(pre.places) + prepared_place<BN>(a.row_start, req) + c / BN;
+      const uint16_t* block = pre.blocks + at * (2 * PLANES * PLANE) + 8 * tid;
+      info = pre.info[at];
+#pragma unroll
+      for (int u = 0; u < PLANES * UNITS; ++u) {
+        tile_dma16(k_lds + (buf * PLANES * PLANE + u * 8 * kTileThreads) * 2, block + u * 8 * kTileThreads);
+        tile_dma16(v_lds + (buf * PLANES * PLANE + u * 8 * kTileThreads) * 2, block + PLANES * PLANE + u * 8 * kTileThreads);
+      }
+      return;
+    }
 #pragma unroll
     for (int u = 0; u < UNITS; ++u) {
       const int r = my_row + u * ROWS, j = min(c + r, j1 - 1);
@@ -255,6 +386,7 @@ __global__ __launch_bounds__(kTileThreads, HDP == 64 && sizeof(T) == 2 ? 3 : HDP
 #pragma unroll
     for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
   float sub = -INFINITY, l = 0.0f;
+  int o_scale = kAnyScale;  // o is times 2^o_scale (prepared tiles)
   if (j0 < j1) {
     look_up(j0);
     bring(j0, 0, 0);
@@ -269,12 +401,71 @@ __global__ __launch_bounds__(kTileThreads, HDP == 64 && sizeof(T) == 2 ? 3 : HDP
     tile_barrier();  // the tile is there, and the buffer of the tile before is free
     const int now = F32 ? 0 : turn, ok_now = turn;
     turn ^= 1;
+    const int2 tile_info = info;
     if (c + BN < j1) {
       bring(c + BN, F32 ? 0 : turn, turn);
       look_up(c + 2 * BN);
     }
     if (!busy) continue;
     const uint16_t *kt = ks[now] + k_at, *vt = vs[now] + v_at;
+    float c2t = c2;
+    if constexpr (PREPARED) {
+      const int ek = __builtin_amdgcn_readfirstlane(tile_info.x), ev = __builtin_amdgcn_readfirstlane(tile_info.y);
+      // scales that differ by more than 2^48 would leave FP32's range in the sums: such a tile is taken from its rows too
+      const bool plain = ek == kNoTile || (o_scale != kAnyScale && ev != kAnyScale && abs(ev - o_scale) > 48);
+      const int to = plain ? 0 : ev == kAnyScale ? o_scale : ev;
+      if (to != o_scale) {
+        if (o_scale != kAnyScale) {
+#pragma unroll
+          for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[d][i] = ldexpf(o[d][i], to - o_scale);
+        }
+        o_scale = to;
+      }
+      if (plain) {
+        // Position by position in FP32, from the rows: both lanes of a pair form its score, each half of the dims.
+        const float* q = a.q + static_cast<long>(first + row) * a.ldq + static_cast<long>(head) * hd;
+#pragma unroll 1
+        for (int j = c; j < min(c + BN, j1); ++j) {
+          const T* kj = static_cast<const T*>(a.kv.k) + (base + j) * a.kv.ldk + static_cast<long>(kvh) * hd;
+          const T* vj = static_cast<const T*>(a.kv.v) + (base + j) * a.kv.ldv + static_cast<long>(kvh) * hd;
+          float part[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll 1
+          for (int d = 8 * h; d < hd; d += 16) {
+            float x[8], y[8];
+            load8(q + d, x);
+            load8(kj + d, y);
+#pragma unroll
+            for (int u = 0; u < 8; ++u) part[u] = fmaf(x[u], y[u], part[u]);
+          }
+          const float s = half_sum(((part[0] + part[1]) + (part[2] + part[3])) + ((part[4] + part[5]) + (part[6] + part[7])));
+          const bool sees = j < seen;
+          const float high = sees ? s * a.c2 - OFFSET : -INFINITY;
+          if (__any(high > sub + kSubSlack)) {
+            const float up = fmaxf(sub, high), al = up == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(sub - up);
+            sub = up;
+            l *= al;
+#pragma unroll
+            for (int d = 0; d < DT; ++d) o[d] *= al;
+          }
+          if (sees) {
+            const float p = __builtin_amdgcn_exp2f(fmaf(s, a.c2, -(sub == -INFINITY ? 0.0f : sub)));
+            if (h == 0) l += p;
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+              for (int g = 0; g < 4; ++g) {  // dims past hd: the row's last ones, not used
+                const T* at = vj + min(32 * d + 8 * g + 4 * h, hd - 4);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[d][4 * g + i] = fmaf(p, static_cast<float>(at[i]), o[d][4 * g + i]);
+              }
+          }
+        }
+        continue;
+      }
+      c2t = ldexpf(a.c2, -e - (ek == kAnyScale ? 0 : ek));
+    }
 
     f16v sc[SUB];
 #pragma unroll
@@ -295,7 +486,7 @@ __global__ __launch_bounds__(kTileThreads, HDP == 64 && sizeof(T) == 2 ? 3 : HDP
         for (int p = 0; p < PLANES; ++p)
 #pragma unroll
           for (int s = 0; s < SUB; ++s)
-            if (sum - p >= 0) sc[s] = mfma32<T>(kf[s][p], qp[k][sum - p], sc[s]);
+            if (sum - p >= 0) sc[s] = mfma32<C>(kf[s][p], qp[k][sum - p], sc[s]);
     }
     if (c + BN > all_see) {
 #pragma unroll
@@ -322,7 +513,7 @@ __global__ __launch_bounds__(kTileThreads, HDP == 64 && sizeof(T) == 2 ? 3 : HDP
     for (int s = 0; s < SUB; ++s)
 #pragma unroll
       for (int i = 0; i < 16; ++i) cm = fmaxf(cm, sc[s][i]);
-    const float high = half_max(cm) * c2 - OFFSET;
+    const float high = half_max(cm) * c2t - OFFSET;
     if (__any(high > sub + kSubSlack)) {
       const float to = fmaxf(sub, high);
       const float al = to == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(sub - to);
@@ -340,11 +531,11 @@ __global__ __launch_bounds__(kTileThreads, HDP == 64 && sizeof(T) == 2 ? 3 : HDP
         float p[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          p[i] = __builtin_amdgcn_exp2f(fmaf(sc[s][8 * half + i], c2, -from));
+          p[i] = __builtin_amdgcn_exp2f(fmaf(sc[s][8 * half + i], c2t, -from));
           sum += p[i];
         }
         u4v pp[NS];
-        split8<T>(p, pp);
+        split8<C>(p, pp);
         constexpr int TURN = DT < 4 ? DT : 4;  // sums taken in turn
 #pragma unroll
         for (int d0 = 0; d0 < DT; d0 += TURN) {
@@ -365,7 +556,7 @@ __global__ __launch_bounds__(kTileThreads, HDP == 64 && sizeof(T) == 2 ? 3 : HDP
             for (int pl = 0; pl < PLANES; ++pl)
 #pragma unroll
               for (int d = 0; d < TURN; ++d)
-                if (ps - pl >= 0) o[d0 + d] = mfma32<T>(vf[d][pl], pp[ps - pl], o[d0 + d]);
+                if (ps - pl >= 0) o[d0 + d] = mfma32<C>(vf[d][pl], pp[ps - pl], o[d0 + d]);
         }
       }
     }
@@ -374,6 +565,14 @@ __global__ __launch_bounds__(kTileThreads, HDP == 64 && sizeof(T) == 2 ? 3 : HDP
 
   // ---- results ---------------------------------------------------------------------------------------------
   l = half_sum(l);
+  if constexpr (PREPARED) {
+    if (o_scale != kAnyScale && o_scale != 0) {
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[d][i] = ldexpf(o[d][i], -o_scale);
+    }
+  }
   bool bad = !(fabsf(l) < INFINITY);
 #pragma unroll
   for (int d = 0; d < DT; ++d)
@@ -425,27 +624,55 @@ __global__ __launch_bounds__(kTileThreads, HDP == 64 && sizeof(T) == 2 ? 3 : HDP
   }
 }
 
-template <class T, int HDP>
-void run_tiles(const AttnTask& t, bool paged, hipStream_t s) {
-  const size_t places = (static_cast<size_t>(t.r.max_rows) * (t.r.H / t.r.KV) + kTilePairs - 1) / kTilePairs + t.r.n_seqs;
+template <class T, int HDP, int SRC>
+void run_tiles(const AttnTask& t, const PrepareArgs& pre, hipStream_t s) {
+  const size_t places = (static_cast<size_t>(t.r.max_rows) * t.group + kTilePairs - 1) / kTilePairs + t.r.n_seqs;
   const dim3 grid(static_cast<unsigned>(places * t.r.KV), t.tile_split.splits);
-  if (paged) attention_tiles_kernel<T, HDP, true><<<grid, kTileThreads, 0, s>>>(t);
-  else attention_tiles_kernel<T, HDP, false><<<grid, kTileThreads, 0, s>>>(t);
+  if constexpr (SRC == kPrepared) attention_prepare_kernel<T, HDP><<<dim3(pre.places, t.r.KV), kTileThreads, 0, s>>>(pre);
+  attention_tiles_kernel<T, HDP, SRC><<<grid, kTileThreads, 0, s>>>(t, pre);
 }
 
+template <class T, int SRC>
+void run_tiles_of(const AttnTask& t, const PrepareArgs& pre, hipStream_t s) {
+  if (t.r.hd <= 64) run_tiles<T, 64, SRC>(t, pre, s);
+  else if (t.r.hd <= 128) run_tiles<T, 128, SRC>(t, pre, s);
+  else run_tiles<T, 256, SRC>(t, pre, s);
+}
+
+// Places of prepared tiles, and the bytes of a tile, for `hd` and `qtype`.
 template <class T>
-void run_tiles_of(const AttnTask& t, bool paged, hipStream_t s) {
-  if (t.r.hd <= 64) run_tiles<T, 64>(t, paged, s);
-  else if (t.r.hd <= 128) run_tiles<T, 128>(t, paged, s);
-  else run_tiles<T, 256>(t, paged, s);
+PreparedShape shape_of(size_t hd) {
+  auto of = [](auto sh) { return PreparedShape{static_cast<size_t>(sh.BN), static_cast<size_t>(2 * sh.PLANES * sh.PLANE * 2)}; };
+  return hd <= 64 ? of(TileShape<T, 64, kPrepared>{}) : hd <= 128 ? of(TileShape<T, 128, kPrepared>{}) : of(TileShape<T, 256, kPrepared>{});
 }
 
 }  // namespace
 
+PreparedShape prepared_shape(size_t hd, int qtype) {
+  return qtype == EF_QTYPE_F32 ? shape_of<float>(hd) : shape_of<__bf16>(hd);
+}
+
 int launch_attention_tiles(const AttnTask& t, int qtype, bool paged, hipStream_t s) {
-  if (qtype == EF_QTYPE_F32) run_tiles_of<float>(t, paged, s);
-  else if (qtype == EF_QTYPE_F16) run_tiles_of<_Float16>(t, paged, s);
-  else run_tiles_of<__bf16>(t, paged, s);
+  const PrepareArgs none{};
+  if (qtype == EF_QTYPE_F32) paged ? run_tiles_of<float, kPages>(t, none, s) : run_tiles_of<float, kRows>(t, none, s);
+  else if (qtype == EF_QTYPE_F16) paged ? run_tiles_of<_Float16, kPages>(t, none, s) : run_tiles_of<_Float16, kRows>(t, none, s);
+  else paged ? run_tiles_of<__bf16, kPages>(t, none, s) : run_tiles_of<__bf16, kRows>(t, none, s);
+  EFH_HIP(hipGetLastError());
+  return EF_HIP_OK;
+}
+
+int launch_attention_prepared(const AttnTask& t, int qtype, void* ws, size_t places, hipStream_t s) {
+  PrepareArgs pre{};
+  pre.kv = t.r.kv;
+  pre.row_start = t.r.row_start;
+  pre.n_seqs = t.r.n_seqs;
+  pre.max_rows = t.r.max_rows;
+  pre.hd = t.r.hd;
+  pre.places = static_cast<int>(places);
+  pre.blocks = static_cast<uint16_t*>(ws);
+  pre.info = reinterpret_cast<int2*>(static_cast<char*>(ws) + places * t.r.KV * prepared_shape(t.r.hd, qtype).bytes);
+  if (qtype == EF_QTYPE_F32) run_tiles_of<float, kPrepared>(t, pre, s);
+  else run_tiles_of<__bf16, kPrepared>(t, pre, s);
   EFH_HIP(hipGetLastError());
   return EF_HIP_OK;
 }

@@ -79,6 +79,18 @@ PagedPlan plan_paged(size_t H, size_t KV, size_t hd, int qtype, size_t n_seqs, s
   return p;
 }
 
+// Packed FP32 and BF16 rows go through the prepared tiles from this many rows on.
+constexpr size_t kPreparedFrom = 1024;
+
+size_t prepared_places(size_t hd, int qtype, size_t n_seqs, size_t max_rows) {
+  if (qtype == EF_QTYPE_F16 || max_rows < kPreparedFrom) return 0;
+  const size_t rows = prepared_shape(hd, qtype).rows;
+  return (max_rows + rows - 1) / rows + n_seqs;
+}
+size_t prepared_bytes(size_t KV, size_t hd, int qtype, size_t n_seqs, size_t max_rows) {
+  return prepared_places(hd, qtype, n_seqs, max_rows) * KV * (prepared_shape(hd, qtype).bytes + 8);
+}
+
 }  // namespace
 }  // namespace efh
 
@@ -143,8 +155,11 @@ int ef_hip_paged_attention(const float* q, size_t ldq, float* out, size_t ldo, s
 
 size_t ef_hip_packed_attention_workspace_bytes(size_t heads, size_t KV, size_t hd, int qtype, size_t n_seqs,
                                                size_t max_rows) {
-  (void)heads, (void)KV, (void)hd, (void)qtype, (void)n_seqs, (void)max_rows;
-  return 0;
+  if (heads < 1 || heads > 65535 || KV < 1 || heads % KV != 0 || hd < 8 || hd > 256 || hd % 8 != 0 || n_seqs < 1 ||
+      n_seqs > (size_t(1) << 20) || max_rows > (size_t(1) << 30) / heads ||
+      (qtype != EF_QTYPE_F32 && qtype != EF_QTYPE_F16 && qtype != EF_QTYPE_BF16))
+    return 0;
+  return prepared_bytes(KV, hd, qtype, n_seqs, max_rows);
 }
 
 int ef_hip_packed_attention(const float* q, size_t ldq, const void* k, size_t ldk, const void* v, size_t ldv, int qtype,
@@ -172,10 +187,13 @@ int ef_hip_packed_attention(const float* q, size_t ldq, const void* k, size_t ld
             "packed_attention: strides and addresses must be multiples of 16 bytes");
   a.c2 = scale * 1.44269504088896340736f;
   a.kv = KvSource{k, v, static_cast<long>(ldk), static_cast<long>(ldv), nullptr, 0, 0, 0, 0};
-  (void)ws, (void)ws_bytes;
+  const size_t need = prepared_bytes(KV, hd, qtype, n_seqs, max_rows);
+  EFH_CHECK(need == 0 || (ws != nullptr && ws_bytes >= need && aligned16(ws)),
+            "packed_attention: the workspace must have ef_hip_packed_attention_workspace_bytes bytes, at a multiple of 16");
   EFH_RC(require_ready());
   if (max_rows == 0) return EF_HIP_OK;
   const AttnTask t = task_of(a);
+  if (need) return launch_attention_prepared(t, qtype, ws, prepared_places(hd, qtype, n_seqs, max_rows), pick(stream));
   return launch_attention_tiles(t, qtype, false, pick(stream));
 }
 

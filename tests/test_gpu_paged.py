@@ -366,7 +366,7 @@ class Paged:
         return out
 
 
-def check(got, want, what=""):
+def check(got, want, what="", worst=WORST):
     """Relative 2-norms per (row, head); rows that see nothing are zero."""
     got, want = got.astype(np.float64), np.asarray(want)
     norm = np.linalg.norm(want, axis=-1)
@@ -375,7 +375,7 @@ def check(got, want, what=""):
     rel = (err / np.where(norm == 0, 1, norm))[norm > 0]
     if rel.size:
         print(f"{what} relative error: worst {rel.max() / U:.1f} u, rms {np.sqrt((rel ** 2).mean()) / U:.1f} u", flush=True)
-        assert rel.max() < WORST and np.sqrt((rel ** 2).mean()) < TYPICAL, what
+        assert rel.max() < worst and np.sqrt((rel ** 2).mean()) < TYPICAL, what
 
 
 SHAPES = [(32, 4, 64), (8, 2, 128), (4, 4, 64), (6, 1, 80), (2, 1, 256), (20, 1, 8), (7, 1, 96), (70, 2, 64)]
@@ -652,6 +652,85 @@ def test_packed_infinities(hip, qtype, value, which):
         assert np.abs(got[150:200, 4:][..., rest] - want[150:200, 4:][..., rest]).max() < 64 * U
     else:
         assert np.array_equal(np.isnan(got[seen]), np.isnan(want[seen]))
+
+
+# Rows enough for FP32 and BF16 keys and values to be prepared as FP16 tiles (1024 and more).
+@pytest.mark.parametrize("qtype", [L.F32, L.BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("H,KV,hd", [(4, 2, 64), (2, 1, 128), (3, 1, 80), (2, 1, 256), (2, 2, 8)])
+@pytest.mark.parametrize("lens", [[1024], [0, 300, 1, 63, 64, 65, 0, 700, 31, 32, 33, 0]])
+def test_packed_prepared(hip, qtype, H, KV, hd, lens):
+    print(f"[case] prepared {qtype} H={H} KV={KV} hd={hd} {lens}", flush=True)
+    p = Packed(hip, hd + len(lens), qtype, H, KV, hd, lens, pad=8)
+    assert hip.packed_attention_workspace_bytes(H, KV, hd, qtype, len(lens), p.rows + 3) > 0
+    check(p.run(), p.want(), f"prepared {qtype} {H}/{KV}/{hd} {lens}")
+
+
+@pytest.mark.parametrize("qtype", [L.F32, L.BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("how", ["tiles", "jumps", "rows", "zeros", "huge", "tiny"])
+def test_packed_prepared_scales(hip, qtype, hd, how):
+    """Keys and values of very different sizes: from tile to tile, past what the sums' scale can follow, from row to row
+    of a tile, tiles and rows of zeros, and whole inputs far from 1 (queries the other way, so that scores stay)."""
+    p = Packed(hip, 71, qtype, 2, 1, hd, [1000, 90])
+    f = torch.ones(p.rows, 1, 1)
+    i = torch.arange(p.rows)
+    if how == "tiles":
+        f = (2.0 ** ((i // 64 * 5) % 23 - 11).double()).float().view(-1, 1, 1)
+    elif how == "jumps":
+        f = (2.0 ** torch.where(i // 64 % 3 == 1, 60.0, torch.where(i // 64 % 3 == 2, -40.0, 0.0)).double()).float().view(-1, 1, 1)
+    elif how == "rows":
+        f = torch.where(i % 37 == 5, 2.0 ** 20, torch.where(i % 41 == 7, 2.0 ** -20, 1.0)).view(-1, 1, 1)
+    elif how == "zeros":
+        f = torch.where((i // 64 % 3 == 0) | (i % 5 == 1), 0.0, 1.0).view(-1, 1, 1)
+    big = {"huge": 2.0 ** 50, "tiny": 2.0 ** -50}.get(how, 1.0)
+    p.k = (p.k.float() * big).to(TORCH[qtype])
+    p.q = p.q * np.float32(1.0 / big)
+    p.v = (p.v.float() * f * big).to(TORCH[qtype])
+    if how == "zeros":
+        p.k = (p.k.float() * f).to(TORCH[qtype])
+    if how == "rows":  # keys of uneven sizes as well, none so large that one position takes all the weight
+        p.k = (p.k.float() * torch.where(i % 29 == 3, 2.0 ** -30, 1.0).view(-1, 1, 1)).to(TORCH[qtype])
+    got, want = p.run(), p.want()
+    assert np.isfinite(got).all()
+    # Where one value row outweighs the others by its size, its weight's own error is the output's: nothing averages it, and
+    # with a small weight nothing cancels it against the sum.  The exponent c2 s - sub of a weight of e^-10 is about -14:
+    # its rounding (half an ulp of 8 .. 16) is 8 u, c2's two roundings (1.5 u relative) make 21 u of it at 14, together
+    # ln 2 (8 + 21) = 20 u; the score's sums and parts are 12 u, exp2 2 u, the sum's and the output's own sums 8 u:
+    # below 48 u.
+    check(got, want, f"scales {how} {qtype} {hd}", worst=48 * U if how in ("tiles", "jumps", "rows") else WORST)
+
+
+@pytest.mark.parametrize("qtype", [L.F32, L.BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("value", [np.inf, -np.inf, np.nan])
+@pytest.mark.parametrize("which", ["k", "v"])
+def test_packed_prepared_infinities(hip, qtype, value, which):
+    p = Packed(hip, 10, qtype, 8, 2, 64, [80, 900, 60])
+    at = 80 + 500
+    (p.k if which == "k" else p.v)[at, 1, 7] = value
+    got, seen = p.run(), np.zeros((p.rows, 8), bool)
+    seen[at:980, 4:] = True
+    with np.errstate(all="ignore"):
+        want = p.want()
+    assert np.isfinite(got[~seen]).all()
+    check(np.where(seen[..., None], 0, got), np.where(seen[..., None], 0, want), f"prepared {which} {value}")
+    if which == "v":
+        assert np.array_equal(got[at:980, 4:, 7], np.full((400, 4), value, np.float32), equal_nan=True)
+        rest = [d for d in range(64) if d != 7]
+        assert np.abs(got[at:980, 4:][..., rest] - want[at:980, 4:][..., rest]).max() < 64 * U
+    else:
+        assert np.array_equal(np.isnan(got[seen]), np.isnan(want[seen]))
+        fine = seen[..., None] & np.isfinite(want)
+        assert np.abs(got[fine] - want[fine]).max(initial=0) < 64 * U
+
+
+def test_packed_workspace_is_checked(hip):
+    p = Packed(hip, 11, L.F32, 4, 2, 64, [1100])
+    p.run()
+    q, k, v, out, start, ws, (ldq, ldk, ldv, n) = p.dev
+    need = hip.packed_attention_workspace_bytes(4, 2, 64, L.F32, 1, n)
+    for small in (Dev(torch.zeros(need - 1, dtype=torch.uint8)), None):
+        with pytest.raises(L.HipError, match="workspace"):
+            hip.packed_attention(q, ldq, k, ldk, v, ldv, L.F32, out, ldq, 4, 2, 64, start, 1, n, 0.125, ws=small)
 
 
 # ---- captured ------------------------------------------------------------------------------------------
