@@ -40,8 +40,16 @@ __global__ __launch_bounds__(kFewWaves * kWave, HDP == 256 ? 1 : (HDP == 64 && N
   const int m = lane & 15, g4 = lane >> 4;
   const int req = blockIdx.x, kvh = blockIdx.y, split = blockIdx.z / t.tiles, tile0 = blockIdx.z - split * t.tiles;
   const int hd = a.hd, G = t.group;
-  const int first = a.row_start[req], n = min(a.row_start[req + 1], a.max_rows) - first;
   const long base = req * a.kv.table_ld;
+  const int sh = a.kv.page_shift, pmask = (1 << sh) - 1;
+  // the first step's pages, whatever the lengths turn out to be (inside the table, and checked before use)
+  int pages[WIDE ? TILES : 1];
+  if constexpr (WIDE) {
+    const long c0 = static_cast<long>(split) * t.few_split.span + wave * KT, width = (a.kv.table_ld << sh) - 1;
+#pragma unroll
+    for (int u = 0; u < TILES; ++u) pages[u] = a.kv.table[base + (min(c0 + 16 * u, width) >> sh)];
+  }
+  const int first = a.row_start[req], n = min(a.row_start[req + 1], a.max_rows) - first;
   const int kv_len = a.kv_len[req];
   const int kv = static_cast<int>(min(static_cast<long>(kv_len), a.kv.table_ld << a.kv.page_shift));
   if (n <= 0 || static_cast<long>(n) * G > t.few_most) return;
@@ -49,7 +57,6 @@ __global__ __launch_bounds__(kFewWaves * kWave, HDP == 256 ? 1 : (HDP == 64 && N
   if (split >= ns) return;
   const int j0 = split * t.few_split.span, j1 = split == t.few_split.splits - 1 ? max(kv, 0) : min(max(kv, 0), j0 + t.few_split.span);
   const int before = kv_len - n;  // row i sees positions 0 .. before + i
-  const int sh = a.kv.page_shift, pmask = (1 << sh) - 1;
   const T *kp = static_cast<const T*>(a.kv.k), *vp = static_cast<const T*>(a.kv.v);
 
   // this lane's dims: K pieces (clamped into the row: the query is zero there), V pieces
@@ -89,7 +96,6 @@ __global__ __launch_bounds__(kFewWaves * kWave, HDP == 256 ? 1 : (HDP == 64 && N
     long off[WIDE ? TILES : 5 * TILES];
     uint32_t held = 0, held_next = 0;
     constexpr uint32_t ALL = WIDE ? (1u << TILES) - 1 : (1u << 4 * TILES) - 1;
-    int pages[WIDE ? TILES : 1];
     auto look_up = [&](int c) {
       if constexpr (WIDE) {
 #pragma unroll
@@ -153,7 +159,7 @@ __global__ __launch_bounds__(kFewWaves * kWave, HDP == 256 ? 1 : (HDP == 64 && N
     constexpr int STEP = kFewWaves * KT;
     int c = j0 + wave * KT;
     if (c < j1) {
-      look_up(c);
+      if (tile != tile0) look_up(c);
       place(c);
       load_k();
       load_v();

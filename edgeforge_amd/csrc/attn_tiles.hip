@@ -41,22 +41,32 @@ __device__ __forceinline__ float half_sum(float v) {
   return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
-// Request r's tiles have the places floor(start[r] G / 128) + r on: at least as many as it needs, without a sum over
-// the requests before it.  The request of place x, by a whole wave.
-__device__ __forceinline__ long tile_place(const RowsArgs& a, int r) {
-  return static_cast<long>(a.row_start[r]) * (a.H / a.KV) / kTilePairs + r;
-}
-__device__ __forceinline__ int request_of_place(const RowsArgs& a, long x) {
+// Tiles have places: request r's are floor(start[r] f / d) + r on (f / d tiles to a row), at least as many as it needs,
+// without a sum over the requests before it.  Whose a place is, by a whole wave (64 requests in one round of loads), with
+// the request's first row and the next one's.
+struct Found {
+  int req, first, next;
+  long tile;  // the place's number among the request's
+};
+__device__ __forceinline__ long place_of(int start, int r, int f, int d) { return static_cast<long>(start) * f / d + r; }
+__device__ __forceinline__ Found find_request(const int32_t* row_start, int n_seqs, int f, int d, long place) {
   const int lane = threadIdx.x & (kWave - 1);
-  int lo = 0, len = a.n_seqs;
-  while (len > 1) {
+  int lo = 0, len = n_seqs;
+  for (;;) {
     const int step = (len + kWave - 1) / kWave, i = lane * step;
-    const uint64_t below = __ballot(i < len && tile_place(a, lo + i) <= x);
-    const int last = max(__popcll(below) - 1, 0) * step;
-    lo += last;
-    len = min(step, len - last);
+    const int start = row_start[min(lo + i, n_seqs)];
+    const uint64_t below = __ballot(i < len && place_of(start, lo + i, f, d) <= place);
+    const int at = max(__popcll(below) - 1, 0);
+    if (step == 1) {
+      const int req = __builtin_amdgcn_readfirstlane(lo + at);
+      Found r{req, __builtin_amdgcn_readlane(start, at), 0, 0};
+      r.next = at < kWave - 1 ? __builtin_amdgcn_readlane(start, at + 1) : row_start[req + 1];
+      r.tile = place - place_of(r.first, req, f, d);
+      return r;
+    }
+    lo += at * step;
+    len = min(step, len - at * step);
   }
-  return __builtin_amdgcn_readfirstlane(lo);
 }
 
 // Where a tile's keys and values come from.
@@ -121,10 +131,6 @@ struct PrepareArgs {
   int2* info;        // [KV][places]: exponents of K and V (kNoTile: marked; kAnyScale: all zero)
 };
 
-// Request r's tiles have the places floor(start[r] / BN) + r on, as the workgroups' places above.
-template <int BN>
-__device__ __forceinline__ long prepared_place(const int32_t* row_start, int r) { return row_start[r] / BN + r; }
-
 template <class T, int HDP>
 __global__ __launch_bounds__(kTileThreads) void attention_prepare_kernel(PrepareArgs a) {
   using Sh = TileShape<T, HDP, kPrepared>;
@@ -132,17 +138,9 @@ __global__ __launch_bounds__(kTileThreads) void attention_prepare_kernel(Prepare
   __shared__ uint32_t most_s[2], least_s[2];
   const int tid = threadIdx.x, kvh = blockIdx.y, chunk = tid % CHUNKS, my_row = tid / CHUNKS;
   const long place = blockIdx.x;
-  int lo = 0;
-  for (int len = a.n_seqs; len > 1;) {  // request_of_place with this kernel's tiles
-    const int step = (len + kWave - 1) / kWave, i = (tid & (kWave - 1)) * step;
-    const uint64_t below = __ballot(i < len && prepared_place<BN>(a.row_start, lo + i) <= place);
-    const int last = max(__popcll(below) - 1, 0) * step;
-    lo += last;
-    len = min(step, len - last);
-  }
-  const int req = __builtin_amdgcn_readfirstlane(lo), first = a.row_start[req];
-  const int n = min(a.row_start[req + 1], a.max_rows) - first;
-  const long c = (place - prepared_place<BN>(a.row_start, req)) * BN;
+  const Found who = find_request(a.row_start, a.n_seqs, 1, BN, place);
+  const int first = who.first, n = min(who.next, a.max_rows) - first;
+  const long c = who.tile * BN;
   if (n <= 0 || c >= n) return;
   if (tid < 2) {
     most_s[tid] = 0;
@@ -233,9 +231,9 @@ __global__ __launch_bounds__(kTileThreads, HDP == 64 && sizeof(T) == 2 ? 3 : HDP
   // the last places first: a request's last rows see the most positions
   const int kvh = blockIdx.x % a.KV;
   const long place = static_cast<long>(gridDim.x / a.KV) - 1 - blockIdx.x / a.KV;
-  const int req = request_of_place(a, place);
-  const int first = a.row_start[req], n = min(a.row_start[req + 1], a.max_rows) - first;
-  const long tile = place - tile_place(a, req);
+  const Found who = find_request(a.row_start, a.n_seqs, G, kTilePairs, place);
+  const int req = who.req, first = who.first, n = min(who.next, a.max_rows) - first;
+  const long tile = who.tile;
   if (n <= 0 || tile * kTilePairs >= static_cast<long>(n) * G || static_cast<long>(n) * G <= t.few_most) return;
   int before, kv;
   long base;
@@ -265,35 +263,6 @@ __global__ __launch_bounds__(kTileThreads, HDP == 64 && sizeof(T) == 2 ? 3 : HDP
   const bool busy = pair0 + 32 * wave < pairs;  // a wave without a pair only stages
   const int all_see = min(before + t.row_of(pair0 + 32 * wave) + 1, kv);  // positions that every row of the wave sees
 
-  u4v qp[KK][NS];
-  float c2 = a.c2;
-  int e = 0;
-  {
-    const float* q = a.q + static_cast<long>(first + row) * a.ldq + static_cast<long>(head) * hd;
-    float top = 0.0f;
-    if constexpr (std::is_same_v<C, _Float16>) {
-#pragma unroll
-      for (int k = 0; k < KK; ++k) {
-        float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-        if (16 * k + 8 * h < hd) load8(q + 16 * k + 8 * h, x);
-#pragma unroll
-        for (int u = 0; u < 8; ++u) top = fmaxf(top, fabsf(x[u]));
-      }
-      e = query_exponent(half_max(top));
-      c2 = ldexpf(c2, -e);
-    }
-#pragma unroll
-    for (int k = 0; k < KK; ++k) {
-      float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-      if (16 * k + 8 * h < hd) load8(q + 16 * k + 8 * h, x);
-      if constexpr (std::is_same_v<C, _Float16>) {
-#pragma unroll
-        for (int u = 0; u < 8; ++u) x[u] = ldexpf(x[u], e);
-      }
-      split8<C>(x, qp[k]);
-    }
-  }
-
   // ---- bringing tiles ------------------------------------------------------------------------------------
   // Unit u of a thread: the chunk at place (tid % CHUNKS) of row tid / CHUNKS + u * 256 / CHUNKS.  16-bit tiles go to
   // LDS by DMA, a tile ahead, in two buffers; FP32 ones through registers, where they are split.  Rows past j1
@@ -317,7 +286,7 @@ __global__ __launch_bounds__(kTileThreads, HDP == 64 && sizeof(T) == 2 ? 3 : HDP
   int2 info = {0, 0};  // of the tile brought last
   auto bring = [&](int c, int buf, int ok_buf) {
     if constexpr (PREPARED) {
-      const long at = kvh * static_cast<long>(pre.places) + prepared_place<BN>(a.row_start, req) + c / BN;
+      const long at = kvh * static_cast<long>(pre.places) + place_of(first, req, 1, BN) + c / BN;
       const uint16_t* block = pre.blocks + at * (2 * PLANES * PLANE) + 8 * tid;
       info = pre.info[at];
 #pragma unroll
@@ -380,6 +349,46 @@ __global__ __launch_bounds__(kTileThreads, HDP == 64 && sizeof(T) == 2 ? 3 : HDP
   const int vq = (lane & 15) / 4, vchunk = 2 * (lane >> 4 & 1) + (lane & 3) / 2;
   const int k_at = col * HDP, v_at = (4 * h + vq) * HDP + 4 * (lane & 1);
 
+  // ---- queries: their loads and the first tile's in flight together ------------------------------------------
+  f4v raw[KK][2];
+  {
+    const float* q = a.q + static_cast<long>(first + row) * a.ldq + static_cast<long>(head) * hd;
+#pragma unroll
+    for (int k = 0; k < KK; ++k)
+#pragma unroll
+      for (int w = 0; w < 2; ++w) raw[k][w] = *reinterpret_cast<const f4v*>(q + min(16 * k + 8 * h, hd - 8) + 4 * w);
+  }
+  if (j0 < j1) {
+    look_up(j0);
+    bring(j0, 0, 0);
+    look_up(j0 + BN);
+  }
+  u4v qp[KK][NS];
+  float c2 = a.c2;
+  int e = 0;
+  {
+    float x[KK][8], top = 0.0f;
+#pragma unroll
+    for (int k = 0; k < KK; ++k)
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        x[k][u] = 16 * k + 8 * h < hd ? raw[k][u / 4][u % 4] : 0.0f;
+        top = fmaxf(top, fabsf(x[k][u]));
+      }
+    if constexpr (std::is_same_v<C, _Float16>) {
+      e = query_exponent(half_max(top));
+      c2 = ldexpf(c2, -e);
+    }
+#pragma unroll
+    for (int k = 0; k < KK; ++k) {
+      if constexpr (std::is_same_v<C, _Float16>) {
+#pragma unroll
+        for (int u = 0; u < 8; ++u) x[k][u] = ldexpf(x[k][u], e);
+      }
+      split8<C>(x[k], qp[k]);
+    }
+  }
+
   f16v o[DT];
 #pragma unroll
   for (int d = 0; d < DT; ++d)
@@ -387,11 +396,6 @@ __global__ __launch_bounds__(kTileThreads, HDP == 64 && sizeof(T) == 2 ? 3 : HDP
     for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
   float sub = -INFINITY, l = 0.0f;
   int o_scale = kAnyScale;  // o is times 2^o_scale (prepared tiles)
-  if (j0 < j1) {
-    look_up(j0);
-    bring(j0, 0, 0);
-    look_up(j0 + BN);
-  }
   int turn = 0;
   for (int c = j0; c < j1; c += BN) {
     if constexpr (F32) {
