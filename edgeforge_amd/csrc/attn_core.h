@@ -234,6 +234,8 @@ struct PreparedShape {
 PreparedShape prepared_shape(size_t hd, int qtype);
 int launch_attention_prepared(const AttnTask& t, int qtype, void* ws, size_t places, hipStream_t s);
 int launch_attention_tiles(const AttnTask& t, int qtype, bool paged, hipStream_t s);
+// few and tiles in one launch (t.few_wide is not used: 16 pairs to a workgroup)
+int launch_attention_mixed(const AttnTask& t, int qtype, hipStream_t s);
 int launch_attention_join(const AttnTask& t, hipStream_t s);
 int launch_attention_few(const AttnTask& t, int qtype, hipStream_t s);
 

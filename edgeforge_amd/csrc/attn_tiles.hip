@@ -1,116 +1,8 @@
-// Attention of many new rows: chunks over pages, and packed prompts.
-//
-// A workgroup takes 128 (row, query head) pairs of one request and KV head, 32 to a wave, and walks the positions
-// they see in tiles of BN: a tile's keys and values are staged in LDS once for all pairs, loaded into registers
-// while the tile before is used.  S^T = K Q^T by v_mfma_f32_32x32x16 puts a pair's scores in its own two lanes (D:
-// positions 8 (i / 4) + 4 h + i % 4, pair lane % 32, h = lane / 32).  The k slots of a product may hold
-// positions in any order, so the weights feed O^T += V^T P^T from the registers they were computed in, against
-// V read transposed from LDS (ds_read_b64_tr_b16: 16 lanes read four positions' rows of 16 dims and get four
-// positions of a dim each).  16-bit parts of the queries and the weights keep FP32's accuracy (attn_core.h); FP32
-// keys and values are split into three parts as they are staged.
-//
-// Masked positions: scores -inf; rows past the last position or without a page are staged as zeros.  Pairs whose
-// sums come out infinite or NaN are computed again by wave_attend, which reads only what each row sees.
-#include <algorithm>
-
-#include "attn_core.h"
+// Attention of many new rows (attn_tiles.h), and the FP16 tiles of packed FP32 and BF16 rows.
+#include "attn_tiles.h"
 
 namespace efh {
 namespace {
-
-typedef float f16v __attribute__((ext_vector_type(16)));
-typedef short s4v __attribute__((ext_vector_type(4)));
-typedef __attribute__((address_space(3))) s4v* lds_s4v;
-
-constexpr int kTileWaves = 4, kTileThreads = kTileWaves * kWave;
-
-template <class T>
-__device__ __forceinline__ f16v mfma32(u4v a, u4v b, f16v c) {
-  if constexpr (std::is_same_v<T, _Float16>)
-    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8v, a), __builtin_bit_cast(h8v, b), c, 0, 0, 0);
-  else
-    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8v, a), __builtin_bit_cast(b8v, b), c, 0, 0, 0);
-}
-
-__device__ __forceinline__ float half_max(float v) {  // over lanes l and l + 32
-  const u2v b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
-}
-__device__ __forceinline__ float half_sum(float v) {
-  const u2v b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
-}
-
-// Tiles have places: request r's are floor(start[r] f / d) + r on (f / d tiles to a row), at least as many as it needs,
-// without a sum over the requests before it.  Whose a place is, by a whole wave (64 requests in one round of loads), with
-// the request's first row and the next one's.
-struct Found {
-  int req, first, next;
-  long tile;  // the place's number among the request's
-};
-__device__ __forceinline__ long place_of(int start, int r, int f, int d) { return static_cast<long>(start) * f / d + r; }
-__device__ __forceinline__ Found find_request(const int32_t* row_start, int n_seqs, int f, int d, long place) {
-  const int lane = threadIdx.x & (kWave - 1);
-  int lo = 0, len = n_seqs;
-  for (;;) {
-    const int step = (len + kWave - 1) / kWave, i = lane * step;
-    const int start = row_start[min(lo + i, n_seqs)];
-    const uint64_t below = __ballot(i < len && place_of(start, lo + i, f, d) <= place);
-    const int at = max(__popcll(below) - 1, 0);
-    if (step == 1) {
-      const int req = __builtin_amdgcn_readfirstlane(lo + at);
-      Found r{req, __builtin_amdgcn_readlane(start, at), 0, 0};
-      r.next = at < kWave - 1 ? __builtin_amdgcn_readlane(start, at + 1) : row_start[req + 1];
-      r.tile = place - place_of(r.first, req, f, d);
-      return r;
-    }
-    lo += at * step;
-    len = min(step, len - at * step);
-  }
-}
-
-// Where a tile's keys and values come from.
-enum Source {
-  kPages,     // a request's pages, in their own type
-  kRows,      // packed rows, in their own type
-  kPrepared,  // packed FP32 or BF16 rows brought to FP16 by attention_prepare_kernel
-};
-
-template <class T, int HDP, int SRC>
-struct TileShape {
-  static constexpr bool F32 = sizeof(T) == 4, PREPARED = SRC == kPrepared;
-  static constexpr int BN = HDP == 256 || (F32 && HDP >= 128) ? 32 : 64;  // positions of a tile
-  static constexpr int PLANES = !F32 ? 1 : PREPARED ? 2 : 3;              // 16-bit planes of a key or value
-  static constexpr int CHUNKS = HDP / 8;                                  // 16-byte chunks of a row
-  static constexpr int PLANE = BN * HDP;                                  // 16-bit values of a plane
-  static constexpr int BUFFERS = F32 && !PREPARED ? 1 : 2;
-  static constexpr int UNITS = PLANE / 8 / kTileThreads;                  // chunks that a thread brings of a plane
-};
-
-// Rows lie in LDS without padding (a DMA instruction writes 1 KB in one piece), their 16-byte chunks in another order in
-// each row, so that what one LDS cycle serves hits all 64 banks: sixteen lanes that read a chunk of sixteen rows
-// (keys), and 32 that read 64 bytes of four rows (values).  Rows of 128 bytes are half the banks wide.
-template <int CHUNKS>
-__device__ __forceinline__ int k_place(int chunk, int row) {
-  return chunk ^ (CHUNKS == 8 ? row >> 1 & 7 : row & (CHUNKS == 16 ? 15 : 7));
-}
-template <int CHUNKS>
-__device__ __forceinline__ int v_place(int chunk, int row) {
-  return chunk ^ (CHUNKS == 8 ? (row & 2) << 1 : (row & 3) << 2);
-}
-
-// 16 bytes per lane from src to LDS at dst + 16 lane, asynchronously (vmcnt).  As asm because the compiler, seeing
-// such a copy, waits for it before every later LDS read; the kernel waits for its tiles itself.  No register is
-// written but m0, which the compiler sets anew before each use.
-__device__ __forceinline__ void tile_dma16(uint32_t dst, const void* src) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(dst), "v"(src) : "memory");
-}
-// This wave's copies arrived and its LDS accesses done, then the barrier.
-__device__ __forceinline__ void tile_barrier() {
-  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-  __builtin_amdgcn_s_barrier();
-  asm volatile("" ::: "memory");
-}
 
 // ---- packed FP32 and BF16 rows as FP16 ---------------------------------------------------------------------
 // A tile of BN rows of one KV head times a power of two that brings its largest value to 2^7 .. 2^15 (its exponent a
@@ -121,16 +13,6 @@ __device__ __forceinline__ void tile_barrier() {
 // what the three-part BF16 split needs six for, and BF16 keys and values two of three.  The tile is written
 // as the kernel's LDS holds it: planes of K, planes of V.
 // Read and written once, in one pass: bound by memory (6001 rows of 4 heads of 64: 12 + 12 MB).
-constexpr int kNoTile = INT32_MIN, kAnyScale = INT32_MAX;
-
-struct PrepareArgs {
-  KvSource kv;
-  const int32_t* row_start;
-  int n_seqs, max_rows, hd, places;
-  uint16_t* blocks;  // [KV][places][2][PLANES][BN][HDP]
-  int2* info;        // [KV][places]: exponents of K and V (kNoTile: marked; kAnyScale: all zero)
-};
-
 template <class T, int HDP>
 __global__ __launch_bounds__(kTileThreads) void attention_prepare_kernel(PrepareArgs a) {
   using Sh = TileShape<T, HDP, kPrepared>;
@@ -212,426 +94,16 @@ __global__ __launch_bounds__(kTileThreads) void attention_prepare_kernel(Prepare
 }
 
 template <class T, int HDP, int SRC>
-__global__ __launch_bounds__(kTileThreads, HDP == 64 && sizeof(T) == 2 ? 3 : HDP <= 128 ? 2 : 1) void attention_tiles_kernel(AttnTask t, PrepareArgs pre) {
-  using Sh = TileShape<T, HDP, SRC>;
-  using C = std::conditional_t<SRC == kPrepared, _Float16, T>;  // what the products are in
-  constexpr bool PAGED = SRC == kPages, PREPARED = SRC == kPrepared, F32 = Sh::F32 && !PREPARED;
-  constexpr int BN = Sh::BN, SUB = BN / 32, PLANES = Sh::PLANES, CHUNKS = Sh::CHUNKS, PLANE = Sh::PLANE, UNITS = Sh::UNITS;
-  constexpr int BUFFERS = Sh::BUFFERS, KK = HDP / 16, DT = HDP / 32, NS = Parts<C>::N;
-  constexpr float OFFSET = Parts<C>::kSubOffset;
-  __shared__ __attribute__((aligned(1024))) uint16_t ks[BUFFERS][PLANES * PLANE];
-  __shared__ __attribute__((aligned(1024))) uint16_t vs[BUFFERS][PLANES * PLANE];
-  __shared__ uint32_t ok_s[2][BN / 4];  // a byte per position: whether a page holds it
-  __shared__ int lost_s;                      // some tile so far had a position without a page
-
-  const RowsArgs& a = t.r;
-  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid & (kWave - 1);
-  const int col = lane & 31, h = lane >> 5;
-  const int G = t.group, hd = a.hd;
+__global__ __launch_bounds__(kTileThreads, (tile_occupancy<T, HDP>())) void attention_tiles_kernel(AttnTask t, PrepareArgs pre) {
+  __shared__ __attribute__((aligned(1024))) TileLds<T, HDP, SRC> lds;
   // the last places first: a request's last rows see the most positions
-  const int kvh = blockIdx.x % a.KV;
-  const long place = static_cast<long>(gridDim.x / a.KV) - 1 - blockIdx.x / a.KV;
-  const Found who = find_request(a.row_start, a.n_seqs, G, kTilePairs, place);
-  const int req = who.req, first = who.first, n = min(who.next, a.max_rows) - first;
-  const long tile = who.tile;
-  if (n <= 0 || tile * kTilePairs >= static_cast<long>(n) * G || static_cast<long>(n) * G <= t.few_most) return;
-  int before, kv;
-  long base;
-  if constexpr (PAGED) {
-    const int kv_len = a.kv_len[req];
-    kv = static_cast<int>(min(static_cast<long>(kv_len), a.kv.table_ld << a.kv.page_shift));
-    before = kv_len - n;
-    base = req * a.kv.table_ld;
-  } else {
-    kv = n;
-    before = 0;
-    base = first;
-  }
-  const int ns = splits_of(kv, t.tile_split), split = blockIdx.y;
-  if (split >= ns) return;
-
-  // ---- this lane's pair --------------------------------------------------------------------------------
-  const int pairs = n * G;  // above few_most, and below 2^31 (checked on the host)
-  const int pair0 = static_cast<int>(tile) * kTilePairs, pair = pair0 + 32 * wave + col;
-  const bool active = pair < pairs;
-  const int row = active ? t.row_of(pair) : 0, head = kvh * G + (active ? pair - row * G : 0);
-  const int seen = active ? min(before + row + 1, kv) : 0;
-  const int tile_last = min(pair0 + kTilePairs, pairs) - 1;
-  // positions: those of the split that the tile's last row sees
-  const int j0 = split * t.tile_split.span;
-  const int j1 = min(split == t.tile_split.splits - 1 ? kv : min(kv, j0 + t.tile_split.span), min(before + t.row_of(tile_last) + 1, kv));
-  const bool busy = pair0 + 32 * wave < pairs;  // a wave without a pair only stages
-  const int all_see = min(before + t.row_of(pair0 + 32 * wave) + 1, kv);  // positions that every row of the wave sees
-
-  // ---- bringing tiles ------------------------------------------------------------------------------------
-  // Unit u of a thread: the chunk at place (tid % CHUNKS) of row tid / CHUNKS + u * 256 / CHUNKS.  16-bit tiles go to
-  // LDS by DMA, a tile ahead, in two buffers; FP32 ones through registers, where they are split.  Rows past j1
-  // repeat the last one, rows without a page the pool's first, dims past hd the row's last ones: all are masked
-  // or multiplied by zero.
-  constexpr int ROWS = kTileThreads / CHUNKS, WORDS = F32 ? 2 : 1;
-  const int my_place = tid % CHUNKS, my_row = tid / CHUNKS;
-  const int k_col = min(8 * k_place<CHUNKS>(my_place, my_row), hd - 8), v_col = min(8 * v_place<CHUNKS>(my_place, my_row), hd - 8);
-  const T *kp = static_cast<const T*>(a.kv.k) + k_col, *vp = static_cast<const T*>(a.kv.v) + (F32 ? k_col : v_col);
-  static_assert(ROWS % (CHUNKS == 32 ? 8 : 16) == 0, "a thread's rows share their places");
-  int page[UNITS];  // of the next tile's rows
-  auto look_up = [&](int c) {
-    if constexpr (PAGED) {
-#pragma unroll
-      for (int u = 0; u < UNITS; ++u) page[u] = a.kv.table[base + (min(c + my_row + u * ROWS, j1 - 1) >> a.kv.page_shift)];
-    }
-  };
-  u4v kr[F32 ? UNITS : 1][WORDS], vr[F32 ? UNITS : 1][WORDS];
-  const uint32_t k_lds = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) void*)ks)) + 1024 * wave;
-  const uint32_t v_lds = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) void*)vs)) + 1024 * wave;
-  int2 info = {0, 0};  // of the tile brought last
-  auto bring = [&](int c, int buf, int ok_buf) {
-    if constexpr (PREPARED) {
-      const long at = kvh * static_cast<long>(pre.places) + place_of(first, req, 1, BN) + c / BN;
-      const uint16_t* block = pre.blocks + at * (2 * PLANES * PLANE) + 8 * tid;
-      info = pre.info[at];
-#pragma unroll
-      for (int u = 0; u < PLANES * UNITS; ++u) {
-        tile_dma16(k_lds + (buf * PLANES * PLANE + u * 8 * kTileThreads) * 2, block + u * 8 * kTileThreads);
-        tile_dma16(v_lds + (buf * PLANES * PLANE + u * 8 * kTileThreads) * 2, block + PLANES * PLANE + u * 8 * kTileThreads);
-      }
-      return;
-    }
-#pragma unroll
-    for (int u = 0; u < UNITS; ++u) {
-      const int r = my_row + u * ROWS, j = min(c + r, j1 - 1);
-      long ko, vo;
-      if constexpr (PAGED) {
-        const bool real = static_cast<uint32_t>(page[u]) < static_cast<uint32_t>(a.kv.n_pages);
-        ko = vo = real ? page[u] * a.kv.page_stride + ((static_cast<long>(kvh) << a.kv.page_shift) + (j & ((1 << a.kv.page_shift) - 1))) * hd : 0;
-        if (my_place == 0) {
-          reinterpret_cast<uint8_t*>(ok_s[ok_buf])[r] = real;
-          if (!real) lost_s = 1;
-        }
-      } else {
-        ko = (base + j) * a.kv.ldk + static_cast<long>(kvh) * hd;
-        vo = (base + j) * a.kv.ldv + static_cast<long>(kvh) * hd;
-      }
-      if constexpr (F32) {
-#pragma unroll
-        for (int w = 0; w < WORDS; ++w) {
-          kr[u][w] = *reinterpret_cast<const u4v*>(kp + ko + 4 * w);
-          vr[u][w] = *reinterpret_cast<const u4v*>(vp + vo + 4 * w);
-        }
-      } else {
-        tile_dma16(k_lds + (buf * PLANE + u * 8 * kTileThreads) * 2, kp + ko);
-        tile_dma16(v_lds + (buf * PLANE + u * 8 * kTileThreads) * 2, vp + vo);
-      }
-    }
-  };
-  auto put = [&]() {  // FP32: the registers' rows into LDS, split
-    if constexpr (F32) {
-#pragma unroll
-      for (int u = 0; u < UNITS; ++u) {
-        const int r = my_row + u * ROWS, chunk = k_place<CHUNKS>(my_place, my_row);
-#pragma unroll
-        for (int which = 0; which < 2; ++which) {
-          const u4v(&x)[WORDS] = which ? vr[u] : kr[u];
-          float f[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(x[i / 4][i % 4]);
-          u4v part[3];
-          split8<float>(f, part);
-          uint16_t* dst = which ? vs[0] + r * HDP + 8 * v_place<CHUNKS>(chunk, r) : ks[0] + r * HDP + 8 * k_place<CHUNKS>(chunk, r);
-#pragma unroll
-          for (int p = 0; p < 3; ++p) *reinterpret_cast<u4v*>(dst + p * PLANE) = part[p];
-        }
-      }
-    }
-  };
-  if (tid == 0) lost_s = 0;
-  __syncthreads();
-  // this lane's reads: keys' row col, chunk 2 k + h; values' rows 4 h + lane % 16 / 4, dims 16 (lane / 16 % 2) + 4 (lane % 4)
-  const int vq = (lane & 15) / 4, vchunk = 2 * (lane >> 4 & 1) + (lane & 3) / 2;
-  const int k_at = col * HDP, v_at = (4 * h + vq) * HDP + 4 * (lane & 1);
-
-  // ---- queries: their loads and the first tile's in flight together ------------------------------------------
-  f4v raw[KK][2];
-  {
-    const float* q = a.q + static_cast<long>(first + row) * a.ldq + static_cast<long>(head) * hd;
-#pragma unroll
-    for (int k = 0; k < KK; ++k)
-#pragma unroll
-      for (int w = 0; w < 2; ++w) raw[k][w] = *reinterpret_cast<const f4v*>(q + min(16 * k + 8 * h, hd - 8) + 4 * w);
-  }
-  if (j0 < j1) {
-    look_up(j0);
-    bring(j0, 0, 0);
-    look_up(j0 + BN);
-  }
-  u4v qp[KK][NS];
-  float c2 = a.c2;
-  int e = 0;
-  {
-    float x[KK][8], top = 0.0f;
-#pragma unroll
-    for (int k = 0; k < KK; ++k)
-#pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        x[k][u] = 16 * k + 8 * h < hd ? raw[k][u / 4][u % 4] : 0.0f;
-        top = fmaxf(top, fabsf(x[k][u]));
-      }
-    if constexpr (std::is_same_v<C, _Float16>) {
-      e = query_exponent(half_max(top));
-      c2 = ldexpf(c2, -e);
-    }
-#pragma unroll
-    for (int k = 0; k < KK; ++k) {
-      if constexpr (std::is_same_v<C, _Float16>) {
-#pragma unroll
-        for (int u = 0; u < 8; ++u) x[k][u] = ldexpf(x[k][u], e);
-      }
-      split8<C>(x[k], qp[k]);
-    }
-  }
-
-  f16v o[DT];
-#pragma unroll
-  for (int d = 0; d < DT; ++d)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
-  float sub = -INFINITY, l = 0.0f;
-  int o_scale = kAnyScale;  // o is times 2^o_scale (prepared tiles)
-  int turn = 0;
-  for (int c = j0; c < j1; c += BN) {
-    if constexpr (F32) {
-      if (c != j0) tile_barrier();  // the tile before is used
-      put();
-    }
-    tile_barrier();  // the tile is there, and the buffer of the tile before is free
-    const int now = F32 ? 0 : turn, ok_now = turn;
-    turn ^= 1;
-    const int2 tile_info = info;
-    if (c + BN < j1) {
-      bring(c + BN, F32 ? 0 : turn, turn);
-      look_up(c + 2 * BN);
-    }
-    if (!busy) continue;
-    const uint16_t *kt = ks[now] + k_at, *vt = vs[now] + v_at;
-    float c2t = c2;
-    if constexpr (PREPARED) {
-      const int ek = __builtin_amdgcn_readfirstlane(tile_info.x), ev = __builtin_amdgcn_readfirstlane(tile_info.y);
-      // scales that differ by more than 2^48 would leave FP32's range in the sums: such a tile is taken from its rows too
-      const bool plain = ek == kNoTile || (o_scale != kAnyScale && ev != kAnyScale && abs(ev - o_scale) > 48);
-      const int to = plain ? 0 : ev == kAnyScale ? o_scale : ev;
-      if (to != o_scale) {
-        if (o_scale != kAnyScale) {
-#pragma unroll
-          for (int d = 0; d < DT; ++d)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) o[d][i] = ldexpf(o[d][i], to - o_scale);
-        }
-        o_scale = to;
-      }
-      if (plain) {
-        // Position by position in FP32, from the rows: both lanes of a pair form its score, each half of the dims.
-        const float* q = a.q + static_cast<long>(first + row) * a.ldq + static_cast<long>(head) * hd;
-#pragma unroll 1
-        for (int j = c; j < min(c + BN, j1); ++j) {
-          const T* kj = static_cast<const T*>(a.kv.k) + (base + j) * a.kv.ldk + static_cast<long>(kvh) * hd;
-          const T* vj = static_cast<const T*>(a.kv.v) + (base + j) * a.kv.ldv + static_cast<long>(kvh) * hd;
-          float part[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-#pragma unroll 1
-          for (int d = 8 * h; d < hd; d += 16) {
-            float x[8], y[8];
-            load8(q + d, x);
-            load8(kj + d, y);
-#pragma unroll
-            for (int u = 0; u < 8; ++u) part[u] = fmaf(x[u], y[u], part[u]);
-          }
-          const float s = half_sum(((part[0] + part[1]) + (part[2] + part[3])) + ((part[4] + part[5]) + (part[6] + part[7])));
-          const bool sees = j < seen;
-          const float high = sees ? s * a.c2 - OFFSET : -INFINITY;
-          if (__any(high > sub + kSubSlack)) {
-            const float up = fmaxf(sub, high), al = up == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(sub - up);
-            sub = up;
-            l *= al;
-#pragma unroll
-            for (int d = 0; d < DT; ++d) o[d] *= al;
-          }
-          if (sees) {
-            const float p = __builtin_amdgcn_exp2f(fmaf(s, a.c2, -(sub == -INFINITY ? 0.0f : sub)));
-            if (h == 0) l += p;
-#pragma unroll
-            for (int d = 0; d < DT; ++d)
-#pragma unroll
-              for (int g = 0; g < 4; ++g) {  // dims past hd: the row's last ones, not used
-                const T* at = vj + min(32 * d + 8 * g + 4 * h, hd - 4);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) o[d][4 * g + i] = fmaf(p, static_cast<float>(at[i]), o[d][4 * g + i]);
-              }
-          }
-        }
-        continue;
-      }
-      c2t = ldexpf(a.c2, -e - (ek == kAnyScale ? 0 : ek));
-    }
-
-    f16v sc[SUB];
-#pragma unroll
-    for (int s = 0; s < SUB; ++s)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) sc[s][i] = 0.0f;
-#pragma unroll
-    for (int k = 0; k < KK; ++k) {
-      u4v kf[SUB][PLANES];
-#pragma unroll
-      for (int s = 0; s < SUB; ++s)
-#pragma unroll
-        for (int p = 0; p < PLANES; ++p)
-          kf[s][p] = *reinterpret_cast<const u4v*>(kt + p * PLANE + 32 * s * HDP + 8 * k_place<CHUNKS>(2 * k + h, col));
-#pragma unroll
-      for (int sum = NS - 1; sum >= 0; --sum)  // the small products first; the sums in turn, as each waits for itself
-#pragma unroll
-        for (int p = 0; p < PLANES; ++p)
-#pragma unroll
-          for (int s = 0; s < SUB; ++s)
-            if (sum - p >= 0) sc[s] = mfma32<C>(kf[s][p], qp[k][sum - p], sc[s]);
-    }
-    if (c + BN > all_see) {
-#pragma unroll
-      for (int s = 0; s < SUB; ++s)
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-          if (c + 32 * s + 8 * (i / 4) + 4 * h + i % 4 >= seen) sc[s][i] = -INFINITY;
-    }
-    if constexpr (PAGED) {
-      if (lost_s) {
-#pragma unroll
-        for (int s = 0; s < SUB; ++s)
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const uint32_t w = ok_s[ok_now][8 * s + 2 * q + h];
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if (!(w >> (8 * i) & 255)) sc[s][4 * q + i] = -INFINITY;
-          }
-      }
-    }
-    float cm = -INFINITY;
-#pragma unroll
-    for (int s = 0; s < SUB; ++s)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) cm = fmaxf(cm, sc[s][i]);
-    const float high = half_max(cm) * c2t - OFFSET;
-    if (__any(high > sub + kSubSlack)) {
-      const float to = fmaxf(sub, high);
-      const float al = to == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(sub - to);
-      sub = to;
-      l *= al;
-#pragma unroll
-      for (int d = 0; d < DT; ++d) o[d] *= al;
-    }
-    const float from = sub == -INFINITY ? 0.0f : sub;
-    float sum = 0.0f;
-#pragma unroll
-    for (int s = 0; s < SUB; ++s) {
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {  // 16 positions: one step of the products
-        float p[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          p[i] = __builtin_amdgcn_exp2f(fmaf(sc[s][8 * half + i], c2t, -from));
-          sum += p[i];
-        }
-        u4v pp[NS];
-        split8<C>(p, pp);
-        constexpr int TURN = DT < 4 ? DT : 4;  // sums taken in turn
-#pragma unroll
-        for (int d0 = 0; d0 < DT; d0 += TURN) {
-          u4v vf[TURN][PLANES];
-#pragma unroll
-          for (int d = 0; d < TURN; ++d)
-#pragma unroll
-            for (int pl = 0; pl < PLANES; ++pl) {
-              uint16_t* at = const_cast<uint16_t*>(vt) + pl * PLANE + (32 * s + 16 * half) * HDP + 8 * v_place<CHUNKS>(4 * (d0 + d) + vchunk, vq);
-              const s4v lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4v)at);
-              const s4v hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4v)(at + 8 * HDP));
-              const u2v lw = __builtin_bit_cast(u2v, lo), hw = __builtin_bit_cast(u2v, hi);
-              vf[d][pl] = u4v{lw[0], lw[1], hw[0], hw[1]};
-            }
-#pragma unroll
-          for (int ps = NS - 1; ps >= 0; --ps)
-#pragma unroll
-            for (int pl = 0; pl < PLANES; ++pl)
-#pragma unroll
-              for (int d = 0; d < TURN; ++d)
-                if (ps - pl >= 0) o[d0 + d] = mfma32<C>(vf[d][pl], pp[ps - pl], o[d0 + d]);
-        }
-      }
-    }
-    l += sum;
-  }
-
-  // ---- results ---------------------------------------------------------------------------------------------
-  l = half_sum(l);
-  if constexpr (PREPARED) {
-    if (o_scale != kAnyScale && o_scale != 0) {
-#pragma unroll
-      for (int d = 0; d < DT; ++d)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) o[d][i] = ldexpf(o[d][i], -o_scale);
-    }
-  }
-  bool bad = !(fabsf(l) < INFINITY);
-#pragma unroll
-  for (int d = 0; d < DT; ++d)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) bad = bad || !(fabsf(o[d][i]) < INFINITY);
-  const bool direct = ns == 1;
-  const long out_row = static_cast<long>(first + row) * a.ldo + static_cast<long>(head) * hd;
-  const long part_row = (static_cast<long>(split) * a.max_rows + first + row) * a.H + head;
-  if (active) {
-    const float inv = direct ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f;
-    float* dst = direct ? a.out + out_row : t.part + part_row * hd;
-#pragma unroll
-    for (int d = 0; d < DT; ++d)
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int dim = 32 * d + 8 * q + 4 * h;
-        if (dim < hd) *reinterpret_cast<f4v*>(dst + dim) = f4v{o[d][4 * q], o[d][4 * q + 1], o[d][4 * q + 2], o[d][4 * q + 3]} * inv;
-      }
-    if (!direct && h == 0) t.stat[part_row] = f2v{sub, l};
-    if (split == 0 && h == 0 && t.count != nullptr) t.count[static_cast<long>(first + row) * a.H + head] = ns;
-  }
-  uint64_t todo = __ballot(bad && active);
-  todo = (todo | todo >> 32) & 0xFFFFFFFFull;
-  tile_barrier();  // the last tile is used
-  float* qs = reinterpret_cast<float*>(ks[0]) + wave * HDP;
-  for (; todo; todo &= todo - 1) {
-    const int who = __ffsll(static_cast<unsigned long long>(todo)) - 1;
-    const int rr = __shfl(row, who, kWave), hh = __shfl(head, who, kWave), lim = min(j1, __shfl(seen, who, kWave));
-    const float* q = a.q + static_cast<long>(first + rr) * a.ldq + static_cast<long>(hh) * hd;
-    for (int d = lane; d < hd; d += kWave) qs[d] = q[d];
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    float sb = -INFINITY, ov[4] = {0, 0, 0, 0};
-    double ll = 0.0;
-    wave_attend<T, PAGED>(a.kv, kvh, hd, base, qs, a.c2, j0, lim, &sb, &ll, ov);
-    ll = wave_sum_d_dpp(ll);
-    const float inv = ll == 0.0 ? 0.0f : static_cast<float>(1.0 / ll);
-    const long to = direct ? static_cast<long>(first + rr) * a.ldo + static_cast<long>(hh) * hd
-                           : (static_cast<long>(split) * a.max_rows + first + rr) * a.H + hh;
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int d = lane + 64 * u;
-      if (d >= hd) continue;
-      if (direct) a.out[to + d] = ov[u] * inv;
-      else t.part[to * hd + d] = ov[u];
-    }
-    if (!direct && lane == 0) t.stat[to] = f2v{sb, static_cast<float>(ll)};
-    __builtin_amdgcn_wave_barrier();
-  }
+  const int kvh = blockIdx.x % t.r.KV;
+  attention_tiles<T, HDP, SRC>(t, pre, lds, kvh, static_cast<long>(gridDim.x / t.r.KV) - 1 - blockIdx.x / t.r.KV, blockIdx.y);
 }
 
 template <class T, int HDP, int SRC>
 void run_tiles(const AttnTask& t, const PrepareArgs& pre, hipStream_t s) {
-  const size_t places = (static_cast<size_t>(t.r.max_rows) * t.group + kTilePairs - 1) / kTilePairs + t.r.n_seqs;
-  const dim3 grid(static_cast<unsigned>(places * t.r.KV), t.tile_split.splits);
+  const dim3 grid(static_cast<unsigned>(tile_places(t) * t.r.KV), t.tile_split.splits);
   if constexpr (SRC == kPrepared) attention_prepare_kernel<T, HDP><<<dim3(pre.places, t.r.KV), kTileThreads, 0, s>>>(pre);
   attention_tiles_kernel<T, HDP, SRC><<<grid, kTileThreads, 0, s>>>(t, pre);
 }

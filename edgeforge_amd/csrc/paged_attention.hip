@@ -66,7 +66,7 @@ PagedPlan plan_paged(size_t H, size_t KV, size_t hd, int qtype, size_t n_seqs, s
   const size_t few_pairs = p.tiles ? std::max<size_t>(kFewPairs, G) : pairs;
   if (p.few) {
     p.few_most = p.tiles ? static_cast<int>(few_pairs) : 0x7FFFFFFF;
-    p.few_wide = few_pairs > kFewPairs && hd <= 128;
+    p.few_wide = !p.tiles && few_pairs > kFewPairs && hd <= 128;
     const size_t per = p.few_wide ? 2 * kFewPairs : kFewPairs;
     p.few_tiles = static_cast<int>((few_pairs + per - 1) / per);
     p.few_split = split_over(n_seqs * KV * p.few_tiles, cus * (hd <= 64 ? 3 : hd <= 128 ? 2 : 1), longest, kFewStep, kFewStep);
@@ -135,6 +135,10 @@ int ef_hip_paged_attention(const float* q, size_t ldq, float* out, size_t ldo, s
   EFH_CHECK(p.bytes == 0 || (ws != nullptr && ws_bytes >= p.bytes && aligned16(ws)),
             "paged_attention: the workspace must have ef_hip_paged_attention_workspace_bytes bytes, at a multiple of 16");
   EFH_CHECK(static_cast<size_t>(p.few_tiles) * p.few_split.splits <= 65535, "paged_attention: too many heads to a KV head");
+  // workgroups of a launch: places of tiles and requests, by KV heads and ranges
+  const double groups = (static_cast<double>(b.max_rows) * heads / pool->KV / kTilePairs + 1 + b.n_seqs) * pool->KV * p.tile_split.splits +
+                        static_cast<double>(b.n_seqs) * pool->KV * p.few_tiles * p.few_split.splits;
+  EFH_CHECK(groups < 2147483647.0, "paged_attention: too many requests, rows and heads for one launch");
   EFH_RC(require_ready());
   if (b.max_rows == 0) return EF_HIP_OK;
   AttnTask t = task_of(a);
@@ -148,8 +152,9 @@ int ef_hip_paged_attention(const float* q, size_t ldq, float* out, size_t ldo, s
   t.stat = reinterpret_cast<f2v*>(t.part + b.max_rows * heads * splits * pool->hd);
   t.count = splits > 1 ? reinterpret_cast<int*>(t.stat + b.max_rows * heads * splits) : nullptr;
   hipStream_t s = pick(stream);
-  if (p.tiles) EFH_RC(launch_attention_tiles(t, pool->qtype, true, s));
-  if (p.few) EFH_RC(launch_attention_few(t, pool->qtype, s));
+  if (p.tiles && p.few) EFH_RC(launch_attention_mixed(t, pool->qtype, s));
+  else if (p.tiles) EFH_RC(launch_attention_tiles(t, pool->qtype, true, s));
+  else EFH_RC(launch_attention_few(t, pool->qtype, s));
   return splits > 1 ? launch_attention_join(t, s) : EF_HIP_OK;
 }
 
@@ -190,6 +195,8 @@ int ef_hip_packed_attention(const float* q, size_t ldq, const void* k, size_t ld
   const size_t need = prepared_bytes(KV, hd, qtype, n_seqs, max_rows);
   EFH_CHECK(need == 0 || (ws != nullptr && ws_bytes >= need && aligned16(ws)),
             "packed_attention: the workspace must have ef_hip_packed_attention_workspace_bytes bytes, at a multiple of 16");
+  EFH_CHECK((static_cast<double>(max_rows) * heads / KV / kTilePairs + 1 + n_seqs) * KV < 2147483647.0,
+            "packed_attention: too many prompts, rows and heads for one launch");
   EFH_RC(require_ready());
   if (max_rows == 0) return EF_HIP_OK;
   const AttnTask t = task_of(a);
