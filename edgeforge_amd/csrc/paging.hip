@@ -18,7 +18,7 @@ namespace {
 // One workgroup: the sums are over at most a few thousand requests, and the stack orders everything.
 // The sums saturate (a saturating sum is associative), so lengths of any size are compared with the
 // bounds without wrapping.
-constexpr int kPlanThreads = 1024, kPlanWaves = kPlanThreads / kWave;
+constexpr int kPlanFew = 256, kPlanThreads = 1024, kPlanWaves = kPlanThreads / kWave;
 
 struct PlanArgs {
   const int32_t *cached, *fresh;
@@ -42,7 +42,14 @@ __device__ __forceinline__ Three operator+(Three a, Three b) {
 }
 
 // Exclusive prefix of v over the workgroup's threads, on top of *carry, which becomes the total so far.
-__device__ __forceinline__ Three scan_block(Three v, Three* carry, Three (*part)[kPlanWaves]) {
+// The barrier waits for LDS only: nobody reads another thread's stores behind it.
+__device__ __forceinline__ void lds_barrier() {
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+template <int WAVES = kPlanWaves>
+__device__ __forceinline__ Three scan_block(Three v, Three* carry, Three (*part)[WAVES]) {
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
   Three in = v;
 #pragma unroll
@@ -51,181 +58,225 @@ __device__ __forceinline__ Three scan_block(Three v, Three* carry, Three (*part)
     if (lane >= o) in = in + u;
   }
   if (lane == kWave - 1) (*part)[wave] = in;
-  __syncthreads();
+  lds_barrier();
   Three before = *carry, all = *carry;
-  for (int w = 0; w < kPlanWaves; ++w) {
-    if (w < wave) before = before + (*part)[w];
-    all = all + (*part)[w];
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) {
+    const Three p = (*part)[w];
+    if (w < wave) before = before + p;
+    all = all + p;
   }
-  __syncthreads();
+  lds_barrier();
   *carry = all;
   const Three up = {__shfl_up(in.rows, 1, kWave), __shfl_up(in.take, 1, kWave), __shfl_up(in.give, 1, kWave)};
   return lane == 0 ? before : before + up;
 }
 
-// Row i's position and slot; rows behind the last one get position 0 and slot -1.
-template <class P>
-__device__ __forceinline__ void fill_row(const PlanArgs& a, P start, int total, int i) {
-  int p = 0;
-  int64_t s = -1;
-  if (i < total) {
-    const int r = request_of(start, a.n_seqs, i);
-    p = a.kv_len[r] - (start[r + 1] - i);
-    const int page = a.table[r * a.table_ld + (p >> a.page_shift)];
-    if (static_cast<uint32_t>(page) < static_cast<uint32_t>(a.n_pages))
-      s = (static_cast<int64_t>(page) << a.page_shift) + (p & ((1 << a.page_shift) - 1));
-  }
-  a.pos[i] = p;
-  a.slot[i] = s;
+// A request's share of the sums, and whether its length is bad.
+struct Share {
+  Three v;
+  int cached, held;
+  bool bad;
+};
+__device__ __forceinline__ Share share_of(const PlanArgs& a, int r) {
+  Share s = {{0, 0, 0}, 0, 0, false};
+  if (r >= a.n_seqs) return s;
+  const int c = a.cached[r], x = a.fresh[r];
+  const long total = static_cast<long>(c) + max(x, 0), mask = (1L << a.page_shift) - 1;
+  s.cached = c;
+  s.bad = c < 0 || total > (a.table_ld << a.page_shift);
+  if (s.bad) return s;
+  s.held = static_cast<int>((c + mask) >> a.page_shift);
+  if (x < 0) return s;
+  s.v.rows = x;
+  s.v.take = static_cast<uint32_t>(((total + mask) >> a.page_shift) - s.held);
+  return s;
 }
-
-constexpr int kPlanLdsSeqs = 4096;
-
-template <bool FILL>
-__global__ __launch_bounds__(kPlanThreads) void page_plan_kernel(PlanArgs a) {
-  __shared__ Three part[kPlanWaves];
-  __shared__ int starts[FILL ? kPlanLdsSeqs + 1 : 1];
-  const int t = threadIdx.x, lane = t & (kWave - 1), wave = t / kWave;
-  const long width = a.table_ld << a.page_shift;  // positions a table row can hold
-  const int n0 = *a.n_free;
-
-  // request r's share, and whether its length is bad
-  auto share = [&](int r, int* cached, int* held, bool* bad) {
-    Three v = {0, 0, 0};
-    *cached = *held = 0;
-    *bad = false;
-    if (r >= a.n_seqs) return v;
-    const int c = a.cached[r], x = a.fresh[r];
-    const long total = static_cast<long>(c) + max(x, 0), mask = (1L << a.page_shift) - 1;
-    *cached = c;
-    *bad = c < 0 || total > width;
-    if (*bad) return v;
-    *held = static_cast<int>((c + mask) >> a.page_shift);
-    if (x < 0) return v;
-    v.rows = x;
-    v.take = static_cast<uint32_t>(((total + mask) >> a.page_shift) - *held);
-    return v;
-  };
-  auto real_page = [&](int page) { return static_cast<uint32_t>(page) < static_cast<uint32_t>(a.n_pages); };
-  // Whole waves walk the table rows of their ended requests: how many pages each gives, or the pages
-  // themselves pushed from stack place `at` on.
-  auto ended_pages = [&](int r, int held, int at, bool push) {
-    const bool mine = r < a.n_seqs && held > 0 && a.fresh[r] < 0;
-    int count = 0;
-    for (uint64_t todo = __ballot(mine); todo; todo &= todo - 1) {
-      const int who = __ffsll(static_cast<unsigned long long>(todo)) - 1;
-      const int rr = __shfl(r, who, kWave), hh = __shfl(held, who, kWave), base = __shfl(at, who, kWave);
-      int found = 0;
-      for (int j0 = 0; j0 < hh; j0 += kWave) {
-        const int page = j0 + lane < hh ? a.table[rr * a.table_ld + j0 + lane] : -1;
-        const uint64_t ok = __ballot(real_page(page));
-        if (push && real_page(page)) a.free_list[base + found + __popcll(ok & ((1ull << lane) - 1))] = page;
-        found += __popcll(ok);
-      }
-      if (lane == who) count = found;
+__device__ __forceinline__ bool real_page(const PlanArgs& a, int page) {
+  return static_cast<uint32_t>(page) < static_cast<uint32_t>(a.n_pages);
+}
+// Whole waves walk the table rows of their ended requests: how many pages each gives, each given page put(at + i, page).
+template <class F>
+__device__ __forceinline__ int ended_pages(const PlanArgs& a, int r, int held, int at, F&& put) {
+  const int lane = threadIdx.x & (kWave - 1);
+  const bool mine = r < a.n_seqs && held > 0 && a.fresh[r] < 0;
+  int count = 0;
+  for (uint64_t todo = __ballot(mine); todo; todo &= todo - 1) {
+    const int who = __ffsll(static_cast<unsigned long long>(todo)) - 1;
+    const int rr = __shfl(r, who, kWave), hh = __shfl(held, who, kWave), base = __shfl(at, who, kWave);
+    int found = 0;
+    for (int j0 = 0; j0 < hh; j0 += kWave) {
+      const int page = j0 + lane < hh ? a.table[rr * a.table_ld + j0 + lane] : -1;
+      const uint64_t ok = __ballot(real_page(a, page));
+      if (real_page(a, page)) put(base + found + __popcll(ok & ((1ull << lane) - 1)), page);
+      found += __popcll(ok);
     }
-    return count;
-  };
-
-  Three total = {0, 0, 0}, mine = {0, 0, 0}, before = {0, 0, 0};
-  int cached = 0, held = 0, n_bad = 0;
-  bool bad = false;
-  for (int r0 = 0; r0 < a.n_seqs; r0 += kPlanThreads) {
-    mine = share(r0 + t, &cached, &held, &bad);
-    n_bad += __syncthreads_count(bad);
-    mine.give = ended_pages(r0 + t, held, 0, false);
-    before = scan_block(mine, &total, &part);
+    if (lane == who) count = found;
   }
-  const bool once = a.n_seqs <= kPlanThreads;  // then cached, held, mine and before stay for the passes below
-
+  return count;
+}
+// Pages taken: each growing request's first by its own thread (a decode step takes one or none), the others by whole
+// waves.  get(k): the page k places below the top of the stack; keep(k, page).
+template <class Get, class Keep>
+__device__ __forceinline__ void take_pages(const PlanArgs& a, int r, int held, uint32_t take, uint32_t before, Get&& get, Keep&& keep) {
+  const int lane = threadIdx.x & (kWave - 1);
+  if (take > 0) {
+    const int page = get(static_cast<int>(before));
+    a.table[r * a.table_ld + held] = page;
+    keep(static_cast<int>(before), page);
+  }
+  for (uint64_t todo = __ballot(take > 1); todo; todo &= todo - 1) {
+    const int who = __ffsll(static_cast<unsigned long long>(todo)) - 1;
+    const int rr = __shfl(r, who, kWave), h = __shfl(held, who, kWave), n = __shfl(static_cast<int>(take), who, kWave);
+    const int k0 = __shfl(static_cast<int>(before), who, kWave);
+    for (int j = 1 + lane; j < n; j += kWave) {
+      const int page = get(k0 + j);
+      a.table[rr * a.table_ld + h + j] = page;
+      keep(k0 + j, page);
+    }
+  }
+}
+// Whether the step fits, and what does not: the same for every thread.
+struct Verdict {
+  bool fits;
+  uint32_t n1;  // free pages after the gifts
+};
+__device__ __forceinline__ Verdict judge(const PlanArgs& a, Three total, int n_bad, int n0) {
   const uint32_t n1 = add_sat(static_cast<uint32_t>(max(n0, 0)), total.give);
   const bool free_bad = n0 < 0 || n0 > a.n_pages || n1 > static_cast<uint32_t>(a.n_pages);
   const uint32_t missing = free_bad || total.take <= n1 ? 0 : total.take - n1;
   const uint32_t over = total.rows > static_cast<uint32_t>(a.max_rows) ? total.rows - a.max_rows : 0;
   const bool fits = !free_bad && missing == 0 && over == 0 && n_bad == 0;
-  if (t == 0) {
+  if (threadIdx.x == 0) {
     a.status[0] = static_cast<int32_t>(min(missing, 0x7FFFFFFFu));
     a.status[1] = n_bad;
     a.status[2] = static_cast<int32_t>(min(over, 0x7FFFFFFFu));
     a.status[3] = free_bad;
     *a.n_free_out = fits ? static_cast<int32_t>(n1 - total.take) : n0;
     a.row_start[a.n_seqs] = fits ? static_cast<int32_t>(total.rows) : 0;
-    if (FILL && a.n_seqs <= kPlanLdsSeqs) starts[a.n_seqs] = fits ? static_cast<int32_t>(total.rows) : 0;
   }
-  if (fits && total.give > 0) {  // uniform over the workgroup
+  return {fits, n1};
+}
+
+// More requests than threads: every sum again in each pass over them.
+__global__ __launch_bounds__(kPlanThreads) void page_plan_kernel(PlanArgs a) {
+  __shared__ Three part[kPlanWaves];
+  const int t = threadIdx.x, n0 = *a.n_free;
+  auto count_only = [](int, int) {};
+  Three total = {0, 0, 0};
+  int n_bad = 0;
+  for (int r0 = 0; r0 < a.n_seqs; r0 += kPlanThreads) {
+    Share s = share_of(a, r0 + t);
+    n_bad += __syncthreads_count(s.bad);
+    s.v.give = ended_pages(a, r0 + t, s.held, 0, count_only);
+    scan_block(s.v, &total, &part);
+  }
+  const Verdict v = judge(a, total, n_bad, n0);
+  if (v.fits && total.give > 0) {
     Three carry = {0, 0, 0};
     for (int r0 = 0; r0 < a.n_seqs; r0 += kPlanThreads) {
-      if (!once) {
-        mine = share(r0 + t, &cached, &held, &bad);
-        mine.give = ended_pages(r0 + t, held, 0, false);
-        before = scan_block(mine, &carry, &part);
-      }
-      ended_pages(r0 + t, held, n0 + static_cast<int>(before.give), true);
+      Share s = share_of(a, r0 + t);
+      s.v.give = ended_pages(a, r0 + t, s.held, 0, count_only);
+      const Three before = scan_block(s.v, &carry, &part);
+      ended_pages(a, r0 + t, s.held, n0 + static_cast<int>(before.give), [&](int at, int page) { a.free_list[at] = page; });
     }
     __syncthreads();  // what was given is there to be taken
   }
-  {
-    Three carry = {0, 0, 0};
-    for (int r0 = 0; r0 < a.n_seqs; r0 += kPlanThreads) {
-      const int r = r0 + t;
-      if (!once) {
-        mine = share(r, &cached, &held, &bad);
-        before = scan_block(mine, &carry, &part);
-      }
-      if (r >= a.n_seqs) continue;
-      const int start = fits ? static_cast<int>(before.rows) : 0;
-      a.row_start[r] = start;
-      if (FILL && a.n_seqs <= kPlanLdsSeqs) starts[r] = start;
-      a.kv_len[r] = !fits ? cached : a.fresh[r] < 0 ? 0 : cached + static_cast<int>(mine.rows);
-    }
-    // pages taken: whole waves over each growing request, whose share may be long
-    if (fits && total.take > 0) {
-      if (once) {
-        for (uint64_t todo = __ballot(mine.take > 0); todo; todo &= todo - 1) {
-          const int who = __ffsll(static_cast<unsigned long long>(todo)) - 1;
-          const int rr = wave * kWave + who;
-          const int n = __shfl(static_cast<int>(mine.take), who, kWave), h = __shfl(held, who, kWave);
-          const int top = static_cast<int>(n1) - 1 - __shfl(static_cast<int>(before.take), who, kWave);
-          for (int j = lane; j < n; j += kWave) a.table[rr * a.table_ld + h + j] = a.free_list[top - j];
-        }
-      } else {
-        Three again = {0, 0, 0};
-        for (int r0 = 0; r0 < a.n_seqs; r0 += kPlanThreads) {
-          // kv_len may be cached itself, which now holds the positions after the step
-          const int r = r0 + t;
-          Three v = {0, 0, 0};
-          int h = 0;
-          if (r < a.n_seqs && a.fresh[r] >= 0) {
-            const int end = a.kv_len[r], c = end - a.fresh[r], mask = (1 << a.page_shift) - 1;
-            h = (c >> a.page_shift) + ((c & mask) != 0);
-            v.take = (end >> a.page_shift) + ((end & mask) != 0) - h;
-          }
-          const Three at = scan_block(v, &again, &part);
-          for (uint64_t todo = __ballot(v.take > 0); todo; todo &= todo - 1) {
-            const int who = __ffsll(static_cast<unsigned long long>(todo)) - 1;
-            const int rr = r0 + wave * kWave + who;
-            const int n = __shfl(static_cast<int>(v.take), who, kWave), hh = __shfl(h, who, kWave);
-            const int top = static_cast<int>(n1) - 1 - __shfl(static_cast<int>(at.take), who, kWave);
-            for (int j = lane; j < n; j += kWave) a.table[rr * a.table_ld + hh + j] = a.free_list[top - j];
-          }
-        }
-      }
-    }
+  Three carry = {0, 0, 0};
+  for (int r0 = 0; r0 < a.n_seqs; r0 += kPlanThreads) {
+    const int r = r0 + t;
+    const Share s = share_of(a, r);
+    const int x = r < a.n_seqs ? a.fresh[r] : 0;
+    const Three before = scan_block(s.v, &carry, &part);
+    if (v.fits)
+      take_pages(a, r, s.held, s.v.take, before.take, [&](int k) { return a.free_list[static_cast<int>(v.n1) - 1 - k]; }, count_only);
+    if (r >= a.n_seqs) continue;
+    a.row_start[r] = v.fits ? static_cast<int>(before.rows) : 0;
+    a.kv_len[r] = !v.fits ? s.cached : x < 0 ? 0 : s.cached + static_cast<int>(s.v.rows);
+  }
+}
+
+// One request to a thread.  The sums are formed once; given pages, taken pages and the requests' starts are kept in LDS
+// too, so that a step waits for memory four times (lengths, ended requests' pages, free pages, the table) and for
+// none of its own stores.
+constexpr int kPlanKept = 2048;  // given and taken pages kept in LDS; beyond, the stores are waited for
+
+template <int THREADS, bool FILL>
+__global__ __launch_bounds__(THREADS) void page_plan_once_kernel(PlanArgs a) {
+  __shared__ Three part[THREADS / kWave];
+  __shared__ int start_s[THREADS + 1], end_s[THREADS], held_s[THREADS], take_s[THREADS], given_s[kPlanKept], taken_s[kPlanKept];
+  __shared__ int bad_s;
+  const int t = threadIdx.x, n0 = __builtin_amdgcn_readfirstlane(*a.n_free);
+  asm volatile("" ::"s"(n0));  // read before the first barrier: n_free_out may be n_free, and is written behind one
+  Share s = share_of(a, t);
+  const int x = t < a.n_seqs ? a.fresh[t] : 0;
+  if (t == 0) bad_s = 0;
+  s.v.give = ended_pages(a, t, s.held, 0, [](int, int) {});
+  lds_barrier();
+  if (s.bad) atomicAdd(&bad_s, 1);
+  Three total = {0, 0, 0};
+  const Three before = scan_block<THREADS / kWave>(s.v, &total, &part);
+  const Verdict v = judge(a, total, bad_s, n0);
+  const bool kept = total.give <= kPlanKept && total.take <= kPlanKept;
+  if (v.fits && total.give > 0)
+    ended_pages(a, t, s.held, static_cast<int>(before.give), [&](int at, int page) {
+      a.free_list[n0 + at] = page;
+      if (at < kPlanKept) given_s[at] = page;
+    });
+  start_s[t] = v.fits ? static_cast<int>(before.rows) : 0;
+  end_s[t] = s.cached + static_cast<int>(s.v.rows);
+  held_s[t] = s.held;
+  take_s[t] = static_cast<int>(before.take) - s.held;
+  if (t == 0) start_s[a.n_seqs] = v.fits ? static_cast<int>(total.rows) : 0;
+  if (kept) lds_barrier();
+  else __syncthreads();
+  if (v.fits)
+    take_pages(a, t, s.held, s.v.take, before.take,
+               [&](int k) {
+                 const int at = static_cast<int>(v.n1) - 1 - k;
+                 return kept && at >= n0 ? given_s[at - n0] : a.free_list[at];
+               },
+               [&](int k, int page) {
+                 if (k < kPlanKept) taken_s[k] = page;
+               });
+  if (t < a.n_seqs) {
+    a.row_start[t] = v.fits ? static_cast<int>(before.rows) : 0;
+    a.kv_len[t] = !v.fits ? s.cached : x < 0 ? 0 : s.cached + static_cast<int>(s.v.rows);
   }
   if constexpr (FILL) {
-    __syncthreads();
-    const int rows = fits ? static_cast<int>(total.rows) : 0;
-    if (a.n_seqs <= kPlanLdsSeqs) {
-      for (int i = t; i < a.max_rows; i += kPlanThreads) fill_row(a, starts, rows, i);
-    } else {
-      for (int i = t; i < a.max_rows; i += kPlanThreads) fill_row(a, a.row_start, rows, i);
+    if (kept) lds_barrier();
+    else __syncthreads();
+    const int rows = v.fits ? static_cast<int>(total.rows) : 0;
+    for (int i = t; i < a.max_rows; i += THREADS) {
+      int p = 0;
+      int64_t slot = -1;
+      if (i < rows) {
+        const int r = request_of(start_s, a.n_seqs, i);
+        p = end_s[r] - (start_s[r + 1] - i);
+        const int b = p >> a.page_shift;
+        const int page = kept && b >= held_s[r] ? taken_s[take_s[r] + b] : a.table[r * a.table_ld + b];
+        if (real_page(a, page)) slot = (static_cast<int64_t>(page) << a.page_shift) + (p & ((1 << a.page_shift) - 1));
+      }
+      a.pos[i] = p;
+      a.slot[i] = slot;
     }
   }
 }
 
+// Each row's position and slot; rows behind the last one get position 0 and slot -1.
 __global__ __launch_bounds__(256) void page_rows_kernel(PlanArgs a) {
   const int i = blockIdx.x * 256 + threadIdx.x;
-  if (i < a.max_rows) fill_row(a, a.row_start, a.row_start[a.n_seqs], i);
+  if (i >= a.max_rows) return;
+  int p = 0;
+  int64_t slot = -1;
+  if (i < a.row_start[a.n_seqs]) {
+    const int r = request_of(a.row_start, a.n_seqs, i);
+    p = a.kv_len[r] - (a.row_start[r + 1] - i);
+    const int page = a.table[r * a.table_ld + (p >> a.page_shift)];
+    if (real_page(a, page)) slot = (static_cast<int64_t>(page) << a.page_shift) + (p & ((1 << a.page_shift) - 1));
+  }
+  a.pos[i] = p;
+  a.slot[i] = slot;
 }
 
 // Rows up to which the plan's own workgroup fills positions and slots.
@@ -373,10 +424,13 @@ int ef_hip_page_plan(const int32_t* cached, const int32_t* fresh, size_t n_seqs,
                    static_cast<int>(max_rows), status};
   EFH_RC(require_ready());
   hipStream_t s = pick(stream);
-  if (max_rows <= static_cast<size_t>(kPlanFillRows)) {
-    page_plan_kernel<true><<<1, kPlanThreads, 0, s>>>(a);
-  } else {
-    page_plan_kernel<false><<<1, kPlanThreads, 0, s>>>(a);
+  const bool fill = n_seqs <= static_cast<size_t>(kPlanThreads) && max_rows <= static_cast<size_t>(kPlanFillRows);
+  if (n_seqs > static_cast<size_t>(kPlanThreads)) page_plan_kernel<<<1, kPlanThreads, 0, s>>>(a);
+  else if (n_seqs > kPlanFew) fill ? page_plan_once_kernel<kPlanThreads, true><<<1, kPlanThreads, 0, s>>>(a)
+                                   : page_plan_once_kernel<kPlanThreads, false><<<1, kPlanThreads, 0, s>>>(a);
+  else fill ? page_plan_once_kernel<kPlanFew, true><<<1, kPlanFew, 0, s>>>(a)
+            : page_plan_once_kernel<kPlanFew, false><<<1, kPlanFew, 0, s>>>(a);
+  if (!fill && max_rows > 0) {
     EFH_HIP(hipGetLastError());
     page_rows_kernel<<<static_cast<unsigned>((max_rows + 255) / 256), 256, 0, s>>>(a);
   }
