@@ -61,7 +61,7 @@ PagedPlan plan_paged(size_t H, size_t KV, size_t hd, int qtype, size_t n_seqs, s
   PagedPlan p;
   const size_t cus = ctx().cu_count > 0 ? ctx().cu_count : 256;
   const size_t G = H / KV, pairs = std::max<size_t>(max_new, 1) * G, longest = std::max<size_t>(max_kv, 1);
-  p.few = pairs <= kFewAlone || n_seqs > 1;
+  p.few = pairs <= kFewAlone || (n_seqs > 1 && G <= kFewAlone);
   p.tiles = pairs > kFewAlone;
   const size_t few_pairs = p.tiles ? std::max<size_t>(kFewPairs, G) : pairs;
   if (p.few) {

@@ -237,3 +237,192 @@ class Engine:
             self.close()
         except Exception:
             pass
+
+
+class PagesShort(RuntimeError):
+    """A step needs more free pages than there are; nothing was changed."""
+
+
+class PagedEngine:
+    """Transformer::forward for requests of different lengths that come and go: a pool of KV pages per
+    layer, block tables and slots planned on the device, and each step's new tokens (one for a request
+    that decodes, a chunk for one whose prompt is brought in) through every product together.
+
+    `seqs` slots hold one request each; step() takes the new tokens of any of them, release() gives a
+    slot's pages back.  After a step, `logits` holds row i's logits [V] on the device for the i-th slot
+    that got tokens (in order of slots): hip.sample and hip.argmax take it from there.  `kv_type` is what
+    the pages hold (F32 as the engine's cache, F16 or BF16 for half the memory and traffic)."""
+
+    def __init__(self, model, pages: int, page_size: int = 16, seqs: int = 64, rows: int = 512, max_seq: int | None = None,
+                 kv_type: int = EL.F32, stream=None):
+        """model: a DeviceModel or an EfqModel (which has to outlive this).  rows: new tokens of one step;
+        max_seq: positions of one request."""
+        H.init()
+        self.model, self.cfg, self.stream = model, model.cfg, stream
+        c = self.cfg
+        if c.hd % 8:
+            raise ValueError("paged attention needs a head size that is a multiple of 8")
+        self.seqs, self.rows, self.page_size, self.pages = seqs, rows, page_size, pages
+        self.max_seq = min(max_seq or c.max_pos, c.max_pos)
+        self.table_ld = -(-self.max_seq // page_size)
+        self.kvd, self.width = c.KV * c.hd, c.D + 2 * c.KV * c.hd
+        if isinstance(model, DeviceModel):
+            w, nrm = model.weights, model.norms
+            self._layers = [({n: w[(l, n)].handle for n in LAYER_MATS}, nrm[(l, "attn")].ptr, nrm[(l, "ffn")].ptr)
+                            for l in range(c.L)]
+            self._embed, self._head, self._final = w["embed"].handle, w["lm_head"].handle, nrm["final"].ptr
+        else:
+            self._layers = []
+            for l in range(c.L):
+                h = model.layer_handles(l)
+                self._layers.append(({n: getattr(h, n) for n in LAYER_MATS}, h.attn_norm_dev, h.ffn_norm_dev))
+            e, m, f = C.c_void_p(), C.c_void_p(), C.c_void_p()
+            EL.call("ef_hip_model_tensors", model.h, C.byref(e), C.byref(m), C.byref(f))
+            self._embed, self._head, self._final = e.value, m.value, f.value
+        self.pools = [H.PagePool(pages, page_size, c.KV, c.hd, kv_type) for _ in range(c.L)]
+        self.cos, self.sin = H.rope_tables(c.rope_theta, c.hd, self.max_seq)
+        i32 = np.int32
+        self.lens = np.zeros(seqs, i32)  # positions of each slot, as on the device
+        self._len, self._new = H.DeviceArray.from_host(self.lens), H.DeviceArray((seqs,), i32)
+        self._table = H.DeviceArray.from_host(np.full((seqs, self.table_ld), -1, i32))
+        self._free = H.DeviceArray.from_host(np.arange(pages, dtype=i32))
+        self._n_free = H.DeviceArray.from_host(np.array([pages], i32))
+        self._start, self._status = H.DeviceArray((seqs + 1,), i32), H.DeviceArray((4,), i32)
+        self._pos, self._slot = H.DeviceArray((rows,), i32), H.DeviceArray((rows,), np.int64)
+        self._ids, self._last = H.DeviceArray((rows,), i32), H.DeviceArray((max(seqs, rows),), i32)
+        self._x, self._qkv = H.DeviceArray((rows, c.D)), H.DeviceArray((rows, self.width))
+        self._ctx, self._act = H.DeviceArray((rows, c.D)), H.DeviceArray((rows, c.F))
+        self._hidden, self.logits = H.DeviceArray((seqs, c.D)), H.DeviceArray((seqs, c.V))
+        self._x_rows = H.Weight(EL.F32, rows, c.D, device=self._x)  # rows of x, to pick some of them
+        self._ws, self._scale = None, float(np.float32(1.0) / np.sqrt(np.float32(c.hd)))
+
+    # ---- one step -------------------------------------------------------------------------------------
+    def step(self, tokens: dict) -> list[int]:
+        """tokens: {slot: new ids}.  Runs them all; returns the slots in the order of `logits`' rows.  Raises
+        PagesShort, with nothing changed, when the pages do not suffice (release some, or wait)."""
+        slots = sorted(tokens)
+        new = np.zeros(self.seqs, np.int32)
+        ids = [np.asarray(tokens[s], np.int32).reshape(-1) for s in slots]
+        for s, t in zip(slots, ids):
+            if not 0 <= s < self.seqs or t.size == 0:
+                raise ValueError(f"slot {s}: no such slot, or no tokens")
+            if self.lens[s] + t.size > self.max_seq:
+                raise ValueError(f"slot {s}: {self.lens[s] + t.size} positions, max_seq is {self.max_seq}")
+            new[s] = t.size
+        n = int(new.sum())
+        if n == 0:
+            return []
+        if n > self.rows:
+            raise ValueError(f"{n} new tokens, {self.rows} rows")
+        self._plan(new)
+        c, s = self.cfg, self.stream
+        flat = np.concatenate(ids)
+        EL.call("ef_hip_memcpy_h2d", self._ids.ptr, flat.ctypes.data, flat.nbytes, H._s(s))
+        max_new, max_kv = int(new.max()), int(self.lens.max())
+        need = H.paged_attention_workspace_bytes(c.H, self.pools[0], self.seqs, n, max_new, max_kv)
+        self._workspace(need)
+
+        def attend(l):
+            b = self._qkv.ptr
+            H.rope_append(b, self.width, b, self.width, c.H, b + 4 * c.D, self.width, b + 4 * (c.D + self.kvd), self.width, n, self._pos,
+                          self.cos, self.sin, self.max_seq, self._slot, self.pools[l], stream=s)
+            H.paged_attention(b, self.width, self._ctx, c.D, c.H, self.pools[l], self._table, self.table_ld, self._start, self._len,
+                              self.seqs, n, max_new, max_kv, self._scale, ws=self._ws, stream=s)
+
+        self._layers_of(n, attend)
+        last = np.cumsum([t.size for t in ids]).astype(np.int32) - 1
+        self._head_of(last, self.logits)
+        return slots
+
+    def release(self, *slots: int) -> None:
+        """The slots' pages back to the pool; the slots are free for other requests."""
+        new = np.zeros(self.seqs, np.int32)
+        new[list(slots)] = -1
+        self._plan(new)
+
+    def free_pages(self) -> int:
+        return int(self._n_free.numpy(self.stream)[0])
+
+    def score(self, windows) -> list[np.ndarray]:
+        """Teacher-forced NLL of ids[p + 1] at every position p of each window (Engine.score, several windows of
+        different lengths in one pass, without pages)."""
+        c, s = self.cfg, self.stream
+        out, at = [None] * len(windows), 0
+        lens = [len(w) - 1 for w in windows]
+        if any(n < 1 or n > min(self.rows, self.max_seq) for n in lens):
+            raise ValueError(f"windows of 2 to {min(self.rows, self.max_seq) + 1} ids")
+        while at < len(windows):  # as many windows as fit the rows
+            group, n = [], 0
+            while at + len(group) < len(windows) and n + lens[at + len(group)] <= self.rows and len(group) < self.seqs:
+                n += lens[at + len(group)]
+                group.append(at + len(group))
+            up = {self._ids: np.concatenate([np.asarray(windows[i][:-1], np.int32) for i in group]),
+                  self._last: np.concatenate([np.asarray(windows[i][1:], np.int32) for i in group]),
+                  self._pos: np.concatenate([np.arange(lens[i], dtype=np.int32) for i in group]),
+                  self._slot: np.full(n, -1, np.int64),
+                  self._start: np.concatenate([[0], np.cumsum([lens[i] for i in group])]).astype(np.int32)}
+            for dev, host in up.items():
+                EL.call("ef_hip_memcpy_h2d", dev.ptr, host.ctypes.data, host.nbytes, H._s(s))
+            self._workspace(H.packed_attention_workspace_bytes(c.H, c.KV, c.hd, EL.F32, len(group), n))
+
+            def attend(l):
+                q = self._qkv.ptr
+                k, v = q + 4 * c.D, q + 4 * (c.D + self.kvd)
+                H.rope_append(q, self.width, q, self.width, c.H, k, self.width, v, self.width, n, self._pos, self.cos, self.sin, self.max_seq,
+                              self._slot, self.pools[0], k_out=k, ldko=self.width, stream=s)
+                H.packed_attention(q, self.width, k, self.width, v, self.width, EL.F32, self._ctx, c.D, c.H, c.KV, c.hd, self._start,
+                                   len(group), n, self._scale, ws=self._ws, stream=s)
+
+            self._layers_of(n, attend)
+            nll = H.DeviceArray((n,), np.float64)
+            for r0 in range(0, n, self.seqs):  # the logits' buffer holds `seqs` rows at a time
+                m = min(self.seqs, n - r0)
+                job = (EL.ef_hip_job * 1)(EL.ef_hip_job(self.logits.ptr, self._head, self._x.at(r0 * c.D)))
+                EL.call("ef_hip_matvec_jobs_rmsnorm", job, 1, self._final, c.eps, m, c.D, c.V, H._s(s))
+                EL.call("ef_hip_neg_log_prob", self.logits.ptr, c.V, m, c.V, self._last.at(r0), nll.at(r0), H._s(s))
+            got, r0 = nll.numpy(s), 0
+            for i in group:
+                out[i] = got[r0:r0 + lens[i]].copy()
+                r0 += lens[i]
+            at += len(group)
+        return out
+
+    # ---- parts ---------------------------------------------------------------------------------------
+    def _plan(self, new: np.ndarray) -> None:
+        s = self.stream
+        EL.call("ef_hip_memcpy_h2d", self._new.ptr, new.ctypes.data, new.nbytes, H._s(s))
+        H.page_plan(self._len, self._new, self.seqs, self.page_size, self.pages, self._table, self.table_ld, self._free, self._n_free,
+                    self._n_free, self._len, self._start, self._pos, self._slot, self.rows, self._status, stream=s)
+        status = self._status.numpy(s)
+        if status[0]:
+            raise PagesShort(f"{status[0]} pages are missing")
+        if status.any():
+            raise RuntimeError(f"page plan refused: {status.tolist()}")
+        self.lens = np.where(new < 0, 0, self.lens + new).astype(np.int32)
+
+    def _workspace(self, need: int) -> None:
+        if need and (self._ws is None or self._ws.nbytes < need):
+            H.sync(self.stream)  # what uses the smaller one is done
+            self._ws = H.DeviceArray((need,), np.uint8)
+
+    def _layers_of(self, n: int, attend) -> None:
+        """The embedding rows of _ids[:n] and every layer over them, in _x."""
+        c, s = self.cfg, H._s(self.stream)
+        x, qkv, ctx, act = self._x.ptr, self._qkv.ptr, self._ctx.ptr, self._act.ptr
+        EL.call("ef_hip_rows_f32", self._embed, self._ids.ptr, n, x, c.D, s)
+        for l, (w, attn_norm, ffn_norm) in enumerate(self._layers):
+            jobs = (EL.ef_hip_job * 3)(EL.ef_hip_job(qkv, w["wq"], x), EL.ef_hip_job(qkv + 4 * c.D, w["wk"], x),
+                                       EL.ef_hip_job(qkv + 4 * (c.D + self.kvd), w["wv"], x))
+            EL.call("ef_hip_matvec_jobs_rmsnorm", jobs, 3, attn_norm, c.eps, n, c.D, self.width, s)
+            attend(l)
+            EL.call("ef_hip_matvec_residual", w["wo"], ctx, x, n, c.D, c.D, s)
+            EL.call("ef_hip_matvec_swiglu", w["w_gate"], w["w_up"], x, ffn_norm, c.eps, act, n, c.D, c.F, s)
+            EL.call("ef_hip_matvec_residual", w["w_down"], act, x, n, c.F, c.D, s)
+
+    def _head_of(self, rows: np.ndarray, logits: H.DeviceArray) -> None:
+        """Final norm and lm_head of the given rows of _x."""
+        c, s = self.cfg, H._s(self.stream)
+        EL.call("ef_hip_memcpy_h2d", self._last.ptr, rows.ctypes.data, rows.nbytes, s)
+        EL.call("ef_hip_rows_f32", self._x_rows.handle, self._last.ptr, rows.size, self._hidden.ptr, c.D, s)
+        job = (EL.ef_hip_job * 1)(EL.ef_hip_job(logits.ptr, self._head, self._hidden.ptr))
+        EL.call("ef_hip_matvec_jobs_rmsnorm", job, 1, self._final, c.eps, rows.size, c.D, c.V, s)
