@@ -9,11 +9,11 @@ namespace {
 
 static_assert(kFewWaves * kWave == kTileThreads, "one launch for both");
 
-template <class T, int HDP, bool WIDE>
-__global__ __launch_bounds__(kTileThreads, (tile_occupancy<T, HDP>())) void attention_mixed_kernel(AttnTask t, unsigned tile_blocks, int places) {
-  constexpr int NT = 1;
+template <class T, int HC, bool WIDE>
+__global__ __launch_bounds__(kTileThreads, (tile_occupancy<T, HC>())) void attention_mixed_kernel(AttnTask t, unsigned tile_blocks, int places) {
+  constexpr int NT = 1, HDP = row_width(HC);
   __shared__ __attribute__((aligned(1024))) union {
-    TileLds<T, HDP, kPages> tiles;
+    TileLds<T, HC, kPages> tiles;
     FewLds<HDP, NT> few;
   } lds;
   unsigned id = blockIdx.x;
@@ -22,7 +22,7 @@ __global__ __launch_bounds__(kTileThreads, (tile_occupancy<T, HDP>())) void atte
     const int split = id / (static_cast<unsigned>(places) * KV);
     id -= static_cast<unsigned>(split) * places * KV;
     const PrepareArgs none{};
-    attention_tiles<T, HDP, kPages>(t, none, lds.tiles, id % KV, places - 1 - static_cast<long>(id / KV), split);
+    attention_tiles<T, HC, kPages>(t, none, lds.tiles, id % KV, places - 1 - static_cast<long>(id / KV), split);
     return;
   }
   id -= tile_blocks;
@@ -32,19 +32,20 @@ __global__ __launch_bounds__(kTileThreads, (tile_occupancy<T, HDP>())) void atte
   attention_few<T, HDP, NT, WIDE>(t, lds.few, id % t.r.n_seqs, id / t.r.n_seqs, split, rest - split * t.tiles);
 }
 
-template <class T, int HDP>
+template <class T, int HC>
 void run_mixed(const AttnTask& t, hipStream_t s) {
   const size_t places = tile_places(t), tile_blocks = places * t.r.KV * t.tile_split.splits;
   const unsigned blocks = static_cast<unsigned>(tile_blocks + static_cast<size_t>(t.r.n_seqs) * t.r.KV * t.tiles * t.few_split.splits);
   if (t.r.kv.page_shift >= 4)
-    attention_mixed_kernel<T, HDP, true><<<blocks, kTileThreads, 0, s>>>(t, static_cast<unsigned>(tile_blocks), static_cast<int>(places));
+    attention_mixed_kernel<T, HC, true><<<blocks, kTileThreads, 0, s>>>(t, static_cast<unsigned>(tile_blocks), static_cast<int>(places));
   else
-    attention_mixed_kernel<T, HDP, false><<<blocks, kTileThreads, 0, s>>>(t, static_cast<unsigned>(tile_blocks), static_cast<int>(places));
+    attention_mixed_kernel<T, HC, false><<<blocks, kTileThreads, 0, s>>>(t, static_cast<unsigned>(tile_blocks), static_cast<int>(places));
 }
 
 template <class T>
 void run_mixed_of(const AttnTask& t, hipStream_t s) {
   if (t.r.hd <= 64) run_mixed<T, 64>(t, s);
+  else if (t.r.hd <= 96) run_mixed<T, 96>(t, s);
   else if (t.r.hd <= 128) run_mixed<T, 128>(t, s);
   else run_mixed<T, 256>(t, s);
 }

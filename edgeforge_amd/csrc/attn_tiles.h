@@ -75,8 +75,12 @@ enum Source {
   kPrepared,  // packed FP32 or BF16 rows brought to FP16 by attention_prepare_kernel
 };
 
-template <class T, int HDP, int SRC>
+// Heads of up to HC dims (64, 96, 128, 256), in rows of a power of two.
+constexpr int row_width(int HC) { return HC == 96 ? 128 : HC; }
+
+template <class T, int HC, int SRC>
 struct TileShape {
+  static constexpr int HDP = row_width(HC);
   static constexpr bool F32 = sizeof(T) == 4, PREPARED = SRC == kPrepared;
   static constexpr int BN = HDP == 256 || (F32 && HDP >= 128) ? 32 : 64;  // positions of a tile
   static constexpr int PLANES = !F32 ? 1 : PREPARED ? 2 : 3;              // 16-bit planes of a key or value
@@ -121,9 +125,9 @@ struct PrepareArgs {
   int2* info;        // [KV][places]: exponents of K and V (kNoTile: marked; kAnyScale: all zero)
 };
 
-template <class T, int HDP, int SRC>
+template <class T, int HC, int SRC>
 struct TileLds {
-  using Sh = TileShape<T, HDP, SRC>;
+  using Sh = TileShape<T, HC, SRC>;
   uint16_t ks[Sh::BUFFERS][Sh::PLANES * Sh::PLANE];
   uint16_t vs[Sh::BUFFERS][Sh::PLANES * Sh::PLANE];
   uint32_t ok[2][Sh::BN / 4];  // a byte per position: whether a page holds it
@@ -131,14 +135,15 @@ struct TileLds {
 };
 
 // One workgroup: the place `place` of KV head `kvh`, range `split`.
-template <class T, int HDP, int SRC>
-__device__ __forceinline__ void attention_tiles(const AttnTask& t, const PrepareArgs& pre, TileLds<T, HDP, SRC>& lds, int kvh, long place,
+template <class T, int HC, int SRC>
+__device__ __forceinline__ void attention_tiles(const AttnTask& t, const PrepareArgs& pre, TileLds<T, HC, SRC>& lds, int kvh, long place,
                                                 int split) {
-  using Sh = TileShape<T, HDP, SRC>;
+  using Sh = TileShape<T, HC, SRC>;
+  constexpr int HDP = Sh::HDP;
   using C = std::conditional_t<SRC == kPrepared, _Float16, T>;  // what the products are in
   constexpr bool PAGED = SRC == kPages, PREPARED = SRC == kPrepared, F32 = Sh::F32 && !PREPARED;
   constexpr int BN = Sh::BN, SUB = BN / 32, PLANES = Sh::PLANES, CHUNKS = Sh::CHUNKS, PLANE = Sh::PLANE, UNITS = Sh::UNITS;
-  constexpr int KK = HDP / 16, DT = HDP / 32, NS = Parts<C>::N;
+  constexpr int KK = HC / 16, DT = HC / 32, NS = Parts<C>::N;
   constexpr float OFFSET = Parts<C>::kSubOffset;
   auto &ks = lds.ks, &vs = lds.vs;
   auto& ok_s = lds.ok;
@@ -550,7 +555,7 @@ inline size_t tile_places(const AttnTask& t) {
   return (static_cast<size_t>(t.r.max_rows) * t.group + kTilePairs - 1) / kTilePairs + t.r.n_seqs;
 }
 // Workgroups of a CU at the kernel's registers and LDS.
-template <class T, int HDP>
-constexpr int tile_occupancy() { return HDP == 64 && sizeof(T) == 2 ? 3 : HDP <= 128 ? 2 : 1; }
+template <class T, int HC>
+constexpr int tile_occupancy() { return HC == 64 && sizeof(T) == 2 ? 3 : HC <= 128 ? 2 : 1; }
 
 }  // namespace efh

@@ -93,24 +93,25 @@ __global__ __launch_bounds__(kTileThreads) void attention_prepare_kernel(Prepare
   }
 }
 
-template <class T, int HDP, int SRC>
-__global__ __launch_bounds__(kTileThreads, (tile_occupancy<T, HDP>())) void attention_tiles_kernel(AttnTask t, PrepareArgs pre) {
-  __shared__ __attribute__((aligned(1024))) TileLds<T, HDP, SRC> lds;
+template <class T, int HC, int SRC>
+__global__ __launch_bounds__(kTileThreads, (tile_occupancy<T, HC>())) void attention_tiles_kernel(AttnTask t, PrepareArgs pre) {
+  __shared__ __attribute__((aligned(1024))) TileLds<T, HC, SRC> lds;
   // the last places first: a request's last rows see the most positions
   const int kvh = blockIdx.x % t.r.KV;
-  attention_tiles<T, HDP, SRC>(t, pre, lds, kvh, static_cast<long>(gridDim.x / t.r.KV) - 1 - blockIdx.x / t.r.KV, blockIdx.y);
+  attention_tiles<T, HC, SRC>(t, pre, lds, kvh, static_cast<long>(gridDim.x / t.r.KV) - 1 - blockIdx.x / t.r.KV, blockIdx.y);
 }
 
-template <class T, int HDP, int SRC>
+template <class T, int HC, int SRC>
 void run_tiles(const AttnTask& t, const PrepareArgs& pre, hipStream_t s) {
   const dim3 grid(static_cast<unsigned>(tile_places(t) * t.r.KV), t.tile_split.splits);
-  if constexpr (SRC == kPrepared) attention_prepare_kernel<T, HDP><<<dim3(pre.places, t.r.KV), kTileThreads, 0, s>>>(pre);
-  attention_tiles_kernel<T, HDP, SRC><<<grid, kTileThreads, 0, s>>>(t, pre);
+  if constexpr (SRC == kPrepared) attention_prepare_kernel<T, row_width(HC)><<<dim3(pre.places, t.r.KV), kTileThreads, 0, s>>>(pre);
+  attention_tiles_kernel<T, HC, SRC><<<grid, kTileThreads, 0, s>>>(t, pre);
 }
 
 template <class T, int SRC>
 void run_tiles_of(const AttnTask& t, const PrepareArgs& pre, hipStream_t s) {
   if (t.r.hd <= 64) run_tiles<T, 64, SRC>(t, pre, s);
+  else if (t.r.hd <= 96) run_tiles<T, 96, SRC>(t, pre, s);
   else if (t.r.hd <= 128) run_tiles<T, 128, SRC>(t, pre, s);
   else run_tiles<T, 256, SRC>(t, pre, s);
 }

@@ -2,6 +2,8 @@
 // Entry points and the choice of kernel.
 #include <algorithm>
 #include <cmath>
+#include <cstdlib>
+#include <cstring>
 
 #include "attn_core.h"
 
@@ -79,11 +81,26 @@ PagedPlan plan_paged(size_t H, size_t KV, size_t hd, int qtype, size_t n_seqs, s
   return p;
 }
 
-// Packed FP32 and BF16 rows go through the prepared tiles from this many rows on.
-constexpr size_t kPreparedFrom = 1024;
+// Whether packed FP32 and BF16 rows go through the prepared tiles: fewer products, one more launch and pass.  By the
+// work, rows times rows of a prompt on average; us from the rows / prepared, 32 heads over 4 of 64 and over 8 of 128:
+//   FP32, 64:   200 rows 15.5 / 15.8, 333 of 9 prompts 11.1 / 14.5, 500 rows 27.8 / 23.9, 1000 of 8 25.6 / 25.6, 2000 rows
+//               111 / 77
+//   FP32, 128:  100 rows 19.1 / 18.0, 500 rows 66.5 / 39.5, 2000 of 20 58 / 49   (80 and 256: ahead from 64 rows)
+//   BF16, 64:   1000 rows 30.2 / 32.5, 1500 of 3 37 / 40, 2000 rows 61.5 / 59.1, 6000 of 4 181 / 144, 9000 rows 804 / 623
+//   BF16, 128:  1000 rows 46 / 57, 2000 rows 102 / 105, 3000 rows 188 / 157, 9000 rows 1443 / 1170
+// EF_HIP_PACKED_ATTENTION=rows|prepared takes one or the other (tests).
+bool prepares(size_t hd, int qtype, size_t n_seqs, size_t max_rows) {
+  if (qtype == EF_QTYPE_F16 || max_rows == 0) return false;
+  if (const char* e = std::getenv("EF_HIP_PACKED_ATTENTION")) {
+    if (std::strcmp(e, "rows") == 0) return false;
+    if (std::strcmp(e, "prepared") == 0) return true;
+  }
+  const double work = static_cast<double>(max_rows) * max_rows / n_seqs;
+  return work >= (qtype == EF_QTYPE_BF16 ? 4194304.0 : hd <= 64 ? 131072.0 : 4096.0);
+}
 
 size_t prepared_places(size_t hd, int qtype, size_t n_seqs, size_t max_rows) {
-  if (qtype == EF_QTYPE_F16 || max_rows < kPreparedFrom) return 0;
+  if (!prepares(hd, qtype, n_seqs, max_rows)) return 0;
   const size_t rows = prepared_shape(hd, qtype).rows;
   return (max_rows + rows - 1) / rows + n_seqs;
 }

@@ -654,11 +654,16 @@ def test_packed_infinities(hip, qtype, value, which):
         assert np.array_equal(np.isnan(got[seen]), np.isnan(want[seen]))
 
 
-# Rows enough for FP32 and BF16 keys and values to be prepared as FP16 tiles (1024 and more).
+# FP32 and BF16 keys and values prepared as FP16 tiles, as they are where there is enough work.
+@pytest.fixture
+def prepared(monkeypatch):
+    monkeypatch.setenv("EF_HIP_PACKED_ATTENTION", "prepared")
+
+
 @pytest.mark.parametrize("qtype", [L.F32, L.BF16], ids=["f32", "bf16"])
 @pytest.mark.parametrize("H,KV,hd", [(4, 2, 64), (2, 1, 128), (3, 1, 80), (2, 1, 256), (2, 2, 8)])
 @pytest.mark.parametrize("lens", [[1024], [0, 300, 1, 63, 64, 65, 0, 700, 31, 32, 33, 0]])
-def test_packed_prepared(hip, qtype, H, KV, hd, lens):
+def test_packed_prepared(hip, prepared, qtype, H, KV, hd, lens):
     print(f"[case] prepared {qtype} H={H} KV={KV} hd={hd} {lens}", flush=True)
     p = Packed(hip, hd + len(lens), qtype, H, KV, hd, lens, pad=8)
     assert hip.packed_attention_workspace_bytes(H, KV, hd, qtype, len(lens), p.rows + 3) > 0
@@ -668,7 +673,7 @@ def test_packed_prepared(hip, qtype, H, KV, hd, lens):
 @pytest.mark.parametrize("qtype", [L.F32, L.BF16], ids=["f32", "bf16"])
 @pytest.mark.parametrize("hd", [64, 128])
 @pytest.mark.parametrize("how", ["tiles", "jumps", "rows", "zeros", "huge", "tiny"])
-def test_packed_prepared_scales(hip, qtype, hd, how):
+def test_packed_prepared_scales(hip, prepared, qtype, hd, how):
     """Keys and values of very different sizes: from tile to tile, past what the sums' scale can follow, from row to row
     of a tile, tiles and rows of zeros, and whole inputs far from 1 (queries the other way, so that scores stay)."""
     p = Packed(hip, 71, qtype, 2, 1, hd, [1000, 90])
@@ -703,7 +708,7 @@ def test_packed_prepared_scales(hip, qtype, hd, how):
 @pytest.mark.parametrize("qtype", [L.F32, L.BF16], ids=["f32", "bf16"])
 @pytest.mark.parametrize("value", [np.inf, -np.inf, np.nan])
 @pytest.mark.parametrize("which", ["k", "v"])
-def test_packed_prepared_infinities(hip, qtype, value, which):
+def test_packed_prepared_infinities(hip, prepared, qtype, value, which):
     p = Packed(hip, 10, qtype, 8, 2, 64, [80, 900, 60])
     at = 80 + 500
     (p.k if which == "k" else p.v)[at, 1, 7] = value
@@ -721,6 +726,26 @@ def test_packed_prepared_infinities(hip, qtype, value, which):
         assert np.array_equal(np.isnan(got[seen]), np.isnan(want[seen]))
         fine = seen[..., None] & np.isfinite(want)
         assert np.abs(got[fine] - want[fine]).max(initial=0) < 64 * U
+
+
+@pytest.mark.parametrize("qtype", [L.F32, L.BF16], ids=["f32", "bf16"])
+def test_packed_rows_and_prepared_agree(hip, monkeypatch, qtype):
+    """Either way of a packed call, on sides of the rule that chooses: the same within both tolerances."""
+    p = Packed(hip, 12, qtype, 4, 2, 64, [500, 30])
+    monkeypatch.setenv("EF_HIP_PACKED_ATTENTION", "rows")
+    assert hip.packed_attention_workspace_bytes(4, 2, 64, qtype, 2, p.rows + 3) == 0
+    a, want = p.run(), p.want()
+    monkeypatch.setenv("EF_HIP_PACKED_ATTENTION", "prepared")
+    b = p.run()
+    check(a, want, f"rows {qtype}")
+    check(b, want, f"prepared {qtype}")
+
+
+def test_long_context_of_one_request(hip):
+    """One request whose positions are cut into more ranges than one wave adds (65 and more), and a few rows of it."""
+    for new, kv, qtype in ((1, 30001, L.F32), (3, 20011, L.F16), (1, 64 * 128 + 1, L.BF16)):
+        p = Paged(hip, 90, qtype, 8, 1, 128, 32, [new], [kv])
+        check(p.run(), p.want(), f"long context {kv} {qtype}")
 
 
 def test_packed_workspace_is_checked(hip):
