@@ -105,15 +105,14 @@ __device__ void wave_attend(const KvSource& src, int g, int hd, long base, const
 //     two: queries are brought to 2^14 .. 2^15 by one that c2 takes back, and p is formed as 2^7 p (the
 //     offset stays in sub), so that what falls below the smallest half is below 2^-31 of the largest.
 //   BF16: 3 parts (8 bits each, truncated, exact in all 24 bits and FP32's range).
-// FP32 pages are split into 3 BF16 parts too where the matrix tiles are large (6 products; what is dropped is below
-// 2^-21 of a product, at random signs).
+// FP32 keys and values are brought to FP16 by a power of two for a tile and split into 2 parts (attn_tiles.h), or
+// multiplied as they are (attn_few.h).
 template <class T>
 struct Parts;
 template <>
 struct Parts<float> {
-  static constexpr int N = 3;
+  static constexpr int N = 1;
   static constexpr float kSubOffset = 0.0f;
-  typedef b8v V;
 };
 template <>
 struct Parts<_Float16> {

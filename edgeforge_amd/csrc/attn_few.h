@@ -54,7 +54,7 @@ __device__ __forceinline__ void attention_few(const AttnTask& t, FewLds<HDP, NT>
 #pragma unroll
     for (int u = 0; u < TILES; ++u) pages[u] = a.kv.table[base + (min(c0 + 16 * u, width) >> sh)];
   }
-  const int first = a.row_start[req], n = min(a.row_start[req + 1], a.max_rows) - first;
+  const int first = max(a.row_start[req], 0), n = min(a.row_start[req + 1], a.max_rows) - first;
   const int kv_len = a.kv_len[req];
   const int kv = static_cast<int>(min(static_cast<long>(kv_len), a.kv.table_ld << a.kv.page_shift));
   if (n <= 0 || static_cast<long>(n) * G > t.few_most) return;

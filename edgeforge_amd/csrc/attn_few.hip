@@ -25,7 +25,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttnTask t) {
   if (at >= step) return;
   const bool in = d < a.hd;
   const float* part = t.part + at * a.hd + (in ? d : 0);
-  const int ns = t.count[at];
+  const int ns = min(t.count[at], most);
   f4v first[kJoinFirst];
 #pragma unroll
   for (int i = 0; i < kJoinFirst; ++i) first[i] = *reinterpret_cast<const f4v*>(part + min(group + i * GROUPS, most - 1) * step * a.hd);

@@ -83,7 +83,7 @@ struct TileShape {
   static constexpr int HDP = row_width(HC);
   static constexpr bool F32 = sizeof(T) == 4, PREPARED = SRC == kPrepared;
   static constexpr int BN = HDP == 256 || (F32 && HDP >= 128) ? 32 : 64;  // positions of a tile
-  static constexpr int PLANES = !F32 ? 1 : PREPARED ? 2 : 3;              // 16-bit planes of a key or value
+  static constexpr int PLANES = F32 ? 2 : 1;                              // 16-bit planes of a key or value
   static constexpr int CHUNKS = HDP / 8;                                  // 16-byte chunks of a row
   static constexpr int PLANE = BN * HDP;                                  // 16-bit values of a plane
   static constexpr int BUFFERS = F32 && !PREPARED ? 1 : 2;
@@ -117,6 +117,16 @@ __device__ __forceinline__ void tile_barrier() {
 
 constexpr int kNoTile = INT32_MIN, kAnyScale = INT32_MAX;
 
+// A tile's exponents from the bits of the largest magnitude of its keys and of its values, and of the smallest among its
+// rows' largest magnitudes (rows of zeros left out).
+__device__ __forceinline__ int2 tile_scales(uint32_t k_most, uint32_t k_least, uint32_t v_most, uint32_t v_least) {
+  const int ek = k_most == 0 ? kAnyScale : (14 + 127 - static_cast<int>(k_most >> 23)) & ~7;
+  const int ev = v_most == 0 ? kAnyScale : (14 + 127 - static_cast<int>(v_most >> 23)) & ~7;
+  const bool marked = k_most >= 0x7F800000u || v_most >= 0x7F800000u || (k_most != 0 && static_cast<int>(k_least >> 23) - 127 + ek < -1) ||
+                      (v_most != 0 && static_cast<int>(v_least >> 23) - 127 + ev < -1);
+  return marked ? int2{kNoTile, kNoTile} : int2{ek, ev};
+}
+
 struct PrepareArgs {
   KvSource kv;
   const int32_t* row_start;
@@ -132,6 +142,7 @@ struct TileLds {
   uint16_t vs[Sh::BUFFERS][Sh::PLANES * Sh::PLANE];
   uint32_t ok[2][Sh::BN / 4];  // a byte per position: whether a page holds it
   int lost;                    // some tile so far had a position without a page
+  u4v sizes[2][kTileWaves];    // FP32: each wave's largest and smallest rows of the tile
 };
 
 // One workgroup: the place `place` of KV head `kvh`, range `split`.
@@ -140,8 +151,9 @@ __device__ __forceinline__ void attention_tiles(const AttnTask& t, const Prepare
                                                 int split) {
   using Sh = TileShape<T, HC, SRC>;
   constexpr int HDP = Sh::HDP;
-  using C = std::conditional_t<SRC == kPrepared, _Float16, T>;  // what the products are in
-  constexpr bool PAGED = SRC == kPages, PREPARED = SRC == kPrepared, F32 = Sh::F32 && !PREPARED;
+  using C = std::conditional_t<SRC == kPrepared || sizeof(T) == 4, _Float16, T>;  // what the products are in
+  // F32: tiles go through registers, where they are scaled and split; SCALED: their values are times a power of two
+  constexpr bool PAGED = SRC == kPages, PREPARED = SRC == kPrepared, F32 = Sh::F32 && !PREPARED, SCALED = F32 || PREPARED;
   constexpr int BN = Sh::BN, SUB = BN / 32, PLANES = Sh::PLANES, CHUNKS = Sh::CHUNKS, PLANE = Sh::PLANE, UNITS = Sh::UNITS;
   constexpr int KK = HC / 16, DT = HC / 32, NS = Parts<C>::N;
   constexpr float OFFSET = Parts<C>::kSubOffset;
@@ -154,9 +166,9 @@ __device__ __forceinline__ void attention_tiles(const AttnTask& t, const Prepare
   const int col = lane & 31, h = lane >> 5;
   const int G = t.group, hd = a.hd;
   const Found who = find_request(a.row_start, a.n_seqs, G, kTilePairs, place);
-  const int req = who.req, first = who.first, n = min(who.next, a.max_rows) - first;
+  const int req = who.req, first = max(who.first, 0), n = min(who.next, a.max_rows) - first;
   const long tile = who.tile;
-  if (n <= 0 || tile * kTilePairs >= static_cast<long>(n) * G || static_cast<long>(n) * G <= t.few_most) return;
+  if (n <= 0 || tile < 0 || tile * kTilePairs >= static_cast<long>(n) * G || static_cast<long>(n) * G <= t.few_most) return;
   int before, kv;
   long base;
   if constexpr (PAGED) {
@@ -203,10 +215,12 @@ __device__ __forceinline__ void attention_tiles(const AttnTask& t, const Prepare
     }
   };
   u4v kr[F32 ? UNITS : 1][WORDS], vr[F32 ? UNITS : 1][WORDS];
+  uint32_t real_rows = 0;  // FP32: units whose row has a page
   const uint32_t k_lds = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) void*)ks)) + 1024 * wave;
   const uint32_t v_lds = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) void*)vs)) + 1024 * wave;
   int2 info = {0, 0};  // of the tile brought last
   auto bring = [&](int c, int buf, int ok_buf) {
+    real_rows = 0;
     if constexpr (PREPARED) {
       const long at = kvh * static_cast<long>(pre.places) + place_of(first, req, 1, BN) + c / BN;
       const uint16_t* block = pre.blocks + at * (2 * PLANES * PLANE) + 8 * tid;
@@ -229,7 +243,9 @@ __device__ __forceinline__ void attention_tiles(const AttnTask& t, const Prepare
           reinterpret_cast<uint8_t*>(ok_s[ok_buf])[r] = real;
           if (!real) lost_s = 1;
         }
+        real_rows |= real ? 1u << u : 0u;
       } else {
+        real_rows |= 1u << u;
         ko = (base + j) * a.kv.ldk + static_cast<long>(kvh) * hd;
         vo = (base + j) * a.kv.ldv + static_cast<long>(kvh) * hd;
       }
@@ -245,7 +261,46 @@ __device__ __forceinline__ void attention_tiles(const AttnTask& t, const Prepare
       }
     }
   };
-  auto put = [&]() {  // FP32: the registers' rows into LDS, split
+  // FP32: the sizes of the tile's rows (as bits: infinities and NaN are the largest), then, behind a barrier, its scales,
+  // and the tile into LDS as rounded halves and what they left.
+  auto measure = [&](int slot) {
+    if constexpr (F32) {
+      u4v found;
+#pragma unroll
+      for (int which = 0; which < 2; ++which) {
+        uint32_t most = 0, least = 0;  // least: of the complements of rows that are not zero
+#pragma unroll
+        for (int u = 0; u < UNITS; ++u) {
+          const u4v(&x)[WORDS] = which ? vr[u] : kr[u];
+          uint32_t top = 0;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) top = max(top, x[i / 4][i % 4] & 0x7FFFFFFFu);
+          top = real_rows >> u & 1 ? top : 0;
+          top = max(top, dpp_self_u<0xB1>(top));
+          top = max(top, dpp_self_u<0x4E>(top));
+          top = max(top, dpp_self_u<0x141>(top));
+          if constexpr (CHUNKS >= 16) top = max(top, dpp_self_u<0x140>(top));
+          if constexpr (CHUNKS >= 32) top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 16, kWave)));
+          most = max(most, top);
+          least = max(least, top ? ~top : 0u);
+        }
+        found[2 * which] = wave_max_u32_dpp(most);
+        found[2 * which + 1] = wave_max_u32_dpp(least);
+      }
+      if (lane == 0) lds.sizes[slot][wave] = found;
+    }
+  };
+  auto scales = [&](int slot) {
+    u4v m = lds.sizes[slot][0];
+#pragma unroll
+    for (int w = 1; w < kTileWaves; ++w)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) m[i] = max(m[i], lds.sizes[slot][w][i]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m[i] = __builtin_amdgcn_readfirstlane(m[i]);
+    return tile_scales(m[0], ~m[1], m[2], ~m[3]);
+  };
+  auto put = [&](int2 sc) {
     if constexpr (F32) {
 #pragma unroll
       for (int u = 0; u < UNITS; ++u) {
@@ -253,14 +308,15 @@ __device__ __forceinline__ void attention_tiles(const AttnTask& t, const Prepare
 #pragma unroll
         for (int which = 0; which < 2; ++which) {
           const u4v(&x)[WORDS] = which ? vr[u] : kr[u];
+          const int e = which ? sc.y : sc.x;
           float f[8];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(x[i / 4][i % 4]);
-          u4v part[3];
-          split8<float>(f, part);
+          for (int i = 0; i < 8; ++i) f[i] = real_rows >> u & 1 ? ldexpf(__uint_as_float(x[i / 4][i % 4]), e == kAnyScale ? 0 : e) : 0.0f;
+          u4v part[2];
+          split8<_Float16>(f, part);
           uint16_t* dst = which ? vs[0] + r * HDP + 8 * v_place<CHUNKS>(chunk, r) : ks[0] + r * HDP + 8 * k_place<CHUNKS>(chunk, r);
 #pragma unroll
-          for (int p = 0; p < 3; ++p) *reinterpret_cast<u4v*>(dst + p * PLANE) = part[p];
+          for (int p = 0; p < 2; ++p) *reinterpret_cast<u4v*>(dst + p * PLANE) = part[p];
         }
       }
     }
@@ -317,12 +373,14 @@ __device__ __forceinline__ void attention_tiles(const AttnTask& t, const Prepare
 #pragma unroll
     for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
   float sub = -INFINITY, l = 0.0f;
-  int o_scale = kAnyScale;  // o is times 2^o_scale (prepared tiles)
+  int o_scale = kAnyScale;  // o is times 2^o_scale (scaled tiles)
   int turn = 0;
   for (int c = j0; c < j1; c += BN) {
     if constexpr (F32) {
-      if (c != j0) tile_barrier();  // the tile before is used
-      put();
+      measure(turn);
+      tile_barrier();  // the tile before is used, and the sizes are there
+      info = scales(turn);
+      if (info.x != kNoTile) put(info);
     }
     tile_barrier();  // the tile is there, and the buffer of the tile before is free
     const int now = F32 ? 0 : turn, ok_now = turn;
@@ -335,7 +393,7 @@ __device__ __forceinline__ void attention_tiles(const AttnTask& t, const Prepare
     if (!busy) continue;
     const uint16_t *kt = ks[now] + k_at, *vt = vs[now] + v_at;
     float c2t = c2;
-    if constexpr (PREPARED) {
+    if constexpr (SCALED) {
       const int ek = __builtin_amdgcn_readfirstlane(tile_info.x), ev = __builtin_amdgcn_readfirstlane(tile_info.y);
       // scales that differ by more than 2^48 would leave FP32's range in the sums: such a tile is taken from its rows too
       const bool plain = ek == kNoTile || (o_scale != kAnyScale && ev != kAnyScale && abs(ev - o_scale) > 48);
@@ -354,8 +412,9 @@ __device__ __forceinline__ void attention_tiles(const AttnTask& t, const Prepare
         const float* q = a.q + static_cast<long>(first + row) * a.ldq + static_cast<long>(head) * hd;
 #pragma unroll 1
         for (int j = c; j < min(c + BN, j1); ++j) {
-          const T* kj = static_cast<const T*>(a.kv.k) + (base + j) * a.kv.ldk + static_cast<long>(kvh) * hd;
-          const T* vj = static_cast<const T*>(a.kv.v) + (base + j) * a.kv.ldv + static_cast<long>(kvh) * hd;
+          long ko, vo;
+          if (!kv_offset<PAGED>(a.kv, kvh, hd, base, j, &ko, &vo)) continue;
+          const T *kj = static_cast<const T*>(a.kv.k) + ko, *vj = static_cast<const T*>(a.kv.v) + vo;
           float part[8] = {0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll 1
           for (int d = 8 * h; d < hd; d += 16) {
@@ -491,7 +550,7 @@ __device__ __forceinline__ void attention_tiles(const AttnTask& t, const Prepare
 
   // ---- results ---------------------------------------------------------------------------------------------
   l = half_sum(l);
-  if constexpr (PREPARED) {
+  if constexpr (SCALED) {
     if (o_scale != kAnyScale && o_scale != 0) {
 #pragma unroll
       for (int d = 0; d < DT; ++d)

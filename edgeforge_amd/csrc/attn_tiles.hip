@@ -21,9 +21,9 @@ __global__ __launch_bounds__(kTileThreads) void attention_prepare_kernel(Prepare
   const int tid = threadIdx.x, kvh = blockIdx.y, chunk = tid % CHUNKS, my_row = tid / CHUNKS;
   const long place = blockIdx.x;
   const Found who = find_request(a.row_start, a.n_seqs, 1, BN, place);
-  const int first = who.first, n = min(who.next, a.max_rows) - first;
+  const int first = max(who.first, 0), n = min(who.next, a.max_rows) - first;
   const long c = who.tile * BN;
-  if (n <= 0 || c >= n) return;
+  if (n <= 0 || c < 0 || c >= n) return;
   if (tid < 2) {
     most_s[tid] = 0;
     least_s[tid] = 0xFFFFFFFFu;
@@ -64,21 +64,14 @@ __global__ __launch_bounds__(kTileThreads) void attention_prepare_kernel(Prepare
     }
   }
   __syncthreads();
-  int e[2];
-  bool marked = false;
-#pragma unroll
-  for (int kv = 0; kv < 2; ++kv) {
-    const uint32_t most = most_s[kv], least = least_s[kv];
-    e[kv] = most == 0 ? kAnyScale : ((14 + 127 - static_cast<int>(most >> 23)) & ~7);
-    marked = marked || most >= 0x7F800000u || (most != 0 && static_cast<int>(least >> 23) - 127 + e[kv] < -1);
-  }
+  const int2 e = tile_scales(most_s[0], least_s[0], most_s[1], least_s[1]);
   const long at = kvh * static_cast<long>(a.places) + place;
-  if (tid == 0) a.info[at] = marked ? int2{kNoTile, kNoTile} : int2{e[0], e[1]};
-  if (marked) return;
+  if (tid == 0) a.info[at] = e;
+  if (e.x == kNoTile) return;
   uint16_t* block = a.blocks + at * (2 * PLANES * PLANE);
 #pragma unroll
   for (int kv = 0; kv < 2; ++kv) {
-    const int scale = e[kv] == kAnyScale ? 0 : e[kv];
+    const int own = kv ? e.y : e.x, scale = own == kAnyScale ? 0 : own;
 #pragma unroll
     for (int u = 0; u < UNITS; ++u) {
       const int r = my_row + u * ROWS;

@@ -13,16 +13,17 @@ namespace efh {
 namespace {
 
 int check_rows(const RowsArgs& a, size_t heads, size_t KV, size_t n_seqs, size_t max_rows, size_t ldq, size_t ldo,
-               float scale, const std::string& w) {
-  EFH_CHECK(a.q && a.out && a.row_start, w + "null pointer");
-  EFH_CHECK(heads >= 1 && heads <= 65535 && KV >= 1 && heads % KV == 0, w + "heads must be a multiple of the KV heads");
-  EFH_CHECK(n_seqs >= 1 && n_seqs <= (size_t(1) << 20), w + "n_seqs must be in [1, 2^20]");
-  EFH_CHECK(max_rows <= (size_t(1) << 30) / heads, w + "too many rows and heads");
+               float scale, const char* who) {
+  auto w = [who](const char* what) { return std::string(who) + what; };
+  EFH_CHECK(a.q && a.out && a.row_start, w("null pointer"));
+  EFH_CHECK(heads >= 1 && heads <= 65535 && KV >= 1 && heads % KV == 0, w("heads must be a multiple of the KV heads"));
+  EFH_CHECK(n_seqs >= 1 && n_seqs <= (size_t(1) << 20), w("n_seqs must be in [1, 2^20]"));
+  EFH_CHECK(max_rows <= (size_t(1) << 30) / heads, w("too many rows and heads"));
   const size_t nq = heads * static_cast<size_t>(a.hd);
-  EFH_CHECK(max_rows <= 1 || (ldq >= nq && ldo >= nq), w + "a row stride is shorter than its row");
+  EFH_CHECK(max_rows <= 1 || (ldq >= nq && ldo >= nq), w("a row stride is shorter than its row"));
   EFH_CHECK(ldq % 4 == 0 && ldo % 4 == 0 && aligned16(a.q) && aligned16(a.out),
-            w + "strides and addresses must be multiples of 16 bytes");
-  EFH_CHECK(scale > 0.0f && std::isfinite(scale), w + "scale must be positive and finite");
+            w("strides and addresses must be multiples of 16 bytes"));
+  EFH_CHECK(scale > 0.0f && std::isfinite(scale), w("scale must be positive and finite"));
   return EF_HIP_OK;
 }
 
@@ -45,7 +46,7 @@ struct PagedPlan {
 };
 constexpr int kFewPairs = 16, kFewAlone = 64;
 constexpr int kFewStep = 128;
-constexpr int kTileStep = 64, kTileSpanLeast = 256;
+constexpr int kTileStep = 64;
 
 // Ranges of positions: as many as make `wgs` workgroups per range about `want` in all, but none shorter than `least`.
 Split split_over(size_t wgs, size_t want, size_t longest, size_t least, size_t step) {
@@ -75,7 +76,7 @@ PagedPlan plan_paged(size_t H, size_t KV, size_t hd, int qtype, size_t n_seqs, s
   }
   if (p.tiles)
     p.tile_split = split_over(std::max<size_t>((max_rows * G + kTilePairs - 1) / kTilePairs * KV, 1),
-                              cus * (hd <= 64 && qtype != EF_QTYPE_F32 ? 3 : hd <= 128 ? 2 : 1), longest, kTileSpanLeast, kTileStep);
+                              cus * (hd <= 64 && qtype != EF_QTYPE_F32 ? 3 : hd <= 128 ? 2 : 1), longest, longest <= 1536 ? 128 : 256, kTileStep);
   const size_t splits = std::max(p.few_split.splits, p.tile_split.splits);
   if (splits > 1) p.bytes = max_rows * H * (splits * (hd + 2) + 1) * sizeof(float);
   return p;

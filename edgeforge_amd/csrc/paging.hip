@@ -1,6 +1,7 @@
 // Paged KV cache: one step's block tables and slot maps from the requests' lengths, and RoPE with the
 // store of keys and values into their pages.  No counterpart in the reference (one contiguous cache).
 #include <cmath>
+#include <new>
 
 #include "paging.h"
 
@@ -381,21 +382,21 @@ void rope_tables_host(float theta, size_t hd, size_t n_pos, std::vector<float>* 
 }
 
 int check_page_pool(const ef_hip_page_pool* p, const char* who) {
-  const std::string w = std::string(who) + ": ";
-  EFH_CHECK(p != nullptr, w + "null page pool");
-  EFH_CHECK(p->k_dev && p->v_dev, w + "null page memory");
+  auto w = [who](const char* what) { return std::string(who) + ": " + what; };
+  EFH_CHECK(p != nullptr, w("null page pool"));
+  EFH_CHECK(p->k_dev && p->v_dev, w("null page memory"));
   EFH_CHECK(p->qtype == EF_QTYPE_F32 || p->qtype == EF_QTYPE_F16 || p->qtype == EF_QTYPE_BF16,
-            w + "pages hold F32, F16 or BF16 values");
-  EFH_CHECK(p->n_pages >= 1 && p->n_pages <= 0x7FFFFFFF, w + "bad page count");
+            w("pages hold F32, F16 or BF16 values"));
+  EFH_CHECK(p->n_pages >= 1 && p->n_pages <= 0x7FFFFFFF, w("bad page count"));
   EFH_CHECK(p->page_size >= 1 && p->page_size <= 1024 && (p->page_size & (p->page_size - 1)) == 0,
-            w + "page_size must be a power of two up to 1024");
-  EFH_CHECK(p->hd >= 8 && p->hd <= 256 && p->hd % 8 == 0, w + "hd must be a multiple of 8 up to 256");
-  EFH_CHECK(p->KV >= 1 && p->KV <= 65535, w + "bad KV head count");
+            w("page_size must be a power of two up to 1024"));
+  EFH_CHECK(p->hd >= 8 && p->hd <= 256 && p->hd % 8 == 0, w("hd must be a multiple of 8 up to 256"));
+  EFH_CHECK(p->KV >= 1 && p->KV <= 65535, w("bad KV head count"));
   const size_t size = p->qtype == EF_QTYPE_F32 ? 4 : 2, least = p->KV * p->page_size * p->hd;
   EFH_CHECK(pool_stride(*p) >= least && pool_stride(*p) * size % 16 == 0 && pool_stride(*p) <= (size_t(1) << 40),
-            w + "page_stride must hold a page and be a multiple of 16 bytes");
-  EFH_CHECK(pool_stride(*p) <= (size_t(1) << 60) / p->n_pages, w + "pool too large");
-  EFH_CHECK(aligned16(p->k_dev) && aligned16(p->v_dev), w + "page memory must be aligned to 16 bytes");
+            w("page_stride must hold a page and be a multiple of 16 bytes"));
+  EFH_CHECK(pool_stride(*p) <= (size_t(1) << 60) / p->n_pages, w("pool too large"));
+  EFH_CHECK(aligned16(p->k_dev) && aligned16(p->v_dev), w("page memory must be aligned to 16 bytes"));
   return EF_HIP_OK;
 }
 
@@ -440,11 +441,15 @@ int ef_hip_page_plan(const int32_t* cached, const int32_t* fresh, size_t n_seqs,
 
 int ef_hip_rope_tables(float theta, size_t hd, size_t n_pos, float* cos_dev, float* sin_dev) {
   EFH_CHECK(cos_dev && sin_dev, "rope_tables: null pointer");
-  EFH_CHECK(theta > 0.0f && hd >= 2 && hd % 2 == 0 && hd <= 4096 && n_pos >= 1 && n_pos <= (size_t(1) << 24),
-            "rope_tables: need theta > 0, an even hd up to 4096 and up to 2^24 positions");
+  EFH_CHECK(theta > 0.0f && hd >= 2 && hd % 2 == 0 && hd <= 4096 && n_pos >= 1 && n_pos <= (size_t(1) << 28) / hd,
+            "rope_tables: need theta > 0, an even hd up to 4096 and at most 2^28 / hd positions");
   EFH_RC(require_ready());
   std::vector<float> c, s;
-  rope_tables_host(theta, hd, n_pos, &c, &s);
+  try {
+    rope_tables_host(theta, hd, n_pos, &c, &s);
+  } catch (const std::bad_alloc&) {
+    return fail(EF_HIP_ENOMEM, "rope_tables: no host memory for the tables");
+  }
   EFH_RC(ef_hip_memcpy_h2d(cos_dev, c.data(), c.size() * 4, nullptr));
   return ef_hip_memcpy_h2d(sin_dev, s.data(), s.size() * 4, nullptr);
 }

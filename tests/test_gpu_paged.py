@@ -540,6 +540,34 @@ def test_scores_with_a_common_part(hip, qtype, offset, new, kv):
     assert rel.max() < WORST + 4 * offset * U
 
 
+@pytest.mark.parametrize("new,kv", [([1, 1], [300, 40]), ([70, 2], [300, 40])])
+def test_offsets_past_32_bits(hip, new, kv):
+    """Pages behind the first 2^32 values of the pool (8 GiB each of K and V): stored there and found again."""
+    KV, hd, page, H = 8, 128, 64, 16
+    per = KV * page * hd
+    n_pages = 2 ** 32 // per + 9
+    p = Paged(hip, 97, L.F16, H, KV, hd, page, new, kv)
+    kp, vp = (torch.empty(n_pages, per, dtype=torch.float16, device="cuda") for _ in range(2))
+    far = [n_pages - 1 - i for i in range(p.n_pages)]  # where each page of the small pool goes
+    for a, b in ((p.kp, kp), (p.vp, vp)):
+        for i, f in enumerate(far):
+            b[f] = a.t[i]
+    p.table = np.where(p.table >= 0, np.array(far)[p.table.clip(0)], -1)
+    pool = hip.PagePool(n_pages, page, KV, hd, L.F16, k=Dev(kp), v=Dev(vp))
+    p.pool = pool
+    check(p.run(), p.want(), f"far pages {new}")
+    # and a store there
+    x = torch.randn(1, (H + 2 * KV) * hd)
+    dx, pos, slot = Dev(x), i32([0]), Dev(torch.tensor([(n_pages - 1) * page + 63]))
+    cos, sin = Dev(torch.ones(1, hd // 2)), Dev(torch.zeros(1, hd // 2))
+    torch.cuda.synchronize()
+    base, w = dx.ptr, (H + 2 * KV) * hd
+    hip.rope_append(base, w, base, w, H, base + 4 * H * hd, w, base + 4 * (H + KV) * hd, w, 1, pos, cos, sin, 1, slot, pool)
+    hip.sync()
+    got = kp[n_pages - 1].view(KV, page, hd)[:, 63].float().cpu()
+    assert torch.equal(got, x[0, H * hd:(H + KV) * hd].view(KV, hd).half().float())
+
+
 def test_repeated_calls_give_the_same_bits(hip):
     for new, kv in (([1] * 5, [900, 3, 77, 2000, 512]), ([1, 90, 1], [900, 400, 33])):
         p = Paged(hip, 60, L.F16, 32, 4, 64, 16, new, kv)
@@ -655,9 +683,11 @@ def test_packed_infinities(hip, qtype, value, which):
 
 
 # FP32 and BF16 keys and values prepared as FP16 tiles, as they are where there is enough work.
-@pytest.fixture
-def prepared(monkeypatch):
-    monkeypatch.setenv("EF_HIP_PACKED_ATTENTION", "prepared")
+# Either way FP32 tiles are scaled and split, before the kernel or in it.
+@pytest.fixture(params=["prepared", "rows"])
+def prepared(request, monkeypatch):
+    monkeypatch.setenv("EF_HIP_PACKED_ATTENTION", request.param)
+    return request.param == "prepared"
 
 
 @pytest.mark.parametrize("qtype", [L.F32, L.BF16], ids=["f32", "bf16"])
@@ -666,7 +696,7 @@ def prepared(monkeypatch):
 def test_packed_prepared(hip, prepared, qtype, H, KV, hd, lens):
     print(f"[case] prepared {qtype} H={H} KV={KV} hd={hd} {lens}", flush=True)
     p = Packed(hip, hd + len(lens), qtype, H, KV, hd, lens, pad=8)
-    assert hip.packed_attention_workspace_bytes(H, KV, hd, qtype, len(lens), p.rows + 3) > 0
+    assert (hip.packed_attention_workspace_bytes(H, KV, hd, qtype, len(lens), p.rows + 3) > 0) == prepared
     check(p.run(), p.want(), f"prepared {qtype} {H}/{KV}/{hd} {lens}")
 
 
@@ -739,6 +769,28 @@ def test_packed_rows_and_prepared_agree(hip, monkeypatch, qtype):
     b = p.run()
     check(a, want, f"rows {qtype}")
     check(b, want, f"prepared {qtype}")
+
+
+@pytest.mark.parametrize("hd", [64, 96, 256])
+@pytest.mark.parametrize("how", ["tiles", "jumps", "rows", "zeros"])
+def test_chunk_scales(hip, hd, how):
+    """FP32 pages whose values' sizes differ from tile to tile, by more than the sums' scale can follow, from row to row,
+    and rows of zeros, with a page lost among them."""
+    p = Paged(hip, 95, L.F32, 4, 2, hd, 16, [90, 1], [420, 200])
+    for r in range(2):
+        for j in range(p.kv[r]):
+            f = {"tiles": 2.0 ** (j // 64 * 5 % 23 - 11), "jumps": (1.0, 2.0 ** 60, 2.0 ** -40)[j // 64 % 3],
+                 "rows": 2.0 ** 20 if j % 37 == 5 else 2.0 ** -20 if j % 41 == 7 else 1.0,
+                 "zeros": 0.0 if j // 64 % 3 == 0 or j % 5 == 1 else 1.0}[how]
+            pg, off = p.place(r, j)
+            for pool, host in ((p.vp, p.v),) + (((p.kp, p.k),) if how == "zeros" else ()):
+                view = pool.t[pg].view(2, 16, hd)
+                view[:, off] *= f
+                host[r][j] *= f
+    lost = {(0, 3)}
+    table = p.table.copy()
+    table[0, 3] = -1
+    check(p.run(table=table), p.want(lost), f"chunk scales {how} {hd}", worst=48 * U if how != "zeros" else WORST)
 
 
 def test_long_context_of_one_request(hip):

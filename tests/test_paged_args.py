@@ -47,7 +47,7 @@ refused = {
                                                     "pos", "slot", "status")] +
         [dict(n_seqs=0), dict(n_seqs=(1 << 20) + 1), dict(page_size=0), dict(page_size=3), dict(page_size=2048), dict(n_pages=0),
          dict(n_pages=1 << 31), dict(ld=0), dict(ld=1 << 28), dict(n_seqs=1 << 20, ld=1 << 12), dict(max_rows=1 << 31)]),
-    "ef_hip_rope_tables": (tables, [dict(theta=0.0), dict(hd=63), dict(hd=0), dict(n_pos=0), dict(cos=None), dict(sin=None)]),
+    "ef_hip_rope_tables": (tables, [dict(theta=0.0), dict(hd=63), dict(hd=0), dict(n_pos=0), dict(n_pos=1 << 23), dict(cos=None), dict(sin=None)]),
     "ef_hip_rope_append": (append, bad_pool + [{k: None} for k in ("q", "q_out", "k", "v", "pos", "cos", "sin", "slot")] +
         [dict(heads=0), dict(ldq=252), dict(ldq=258), dict(ldqo=255), dict(ldk=124), dict(ldv=127), dict(k_out=P + 64, ldko=64),
          dict(k_out=P + 4, ldko=128), dict(q=P + 4), dict(q_out=P + 8), dict(k=P + 4), dict(v=P + 12), dict(cos=P + 4), dict(n_pos=0),
