@@ -96,45 +96,57 @@ __device__ __forceinline__ Share share_of(const PlanArgs& a, int r) {
 __device__ __forceinline__ bool real_page(const PlanArgs& a, int page) {
   return static_cast<uint32_t>(page) < static_cast<uint32_t>(a.n_pages);
 }
-// Whole waves walk the table rows of their ended requests: how many pages each gives, each given page put(at + i, page).
+// Whole waves walk the table rows of their ended requests, four pieces of 64 entries in flight: how many pages each
+// request gives, each given page put(at + i, page).
 template <class F>
 __device__ __forceinline__ int ended_pages(const PlanArgs& a, int r, int held, int at, F&& put) {
+  constexpr int FLIGHT = 4;
   const int lane = threadIdx.x & (kWave - 1);
-  const bool mine = r < a.n_seqs && held > 0 && a.fresh[r] < 0;
-  int count = 0;
-  for (uint64_t todo = __ballot(mine); todo; todo &= todo - 1) {
-    const int who = __ffsll(static_cast<unsigned long long>(todo)) - 1;
-    const int rr = __shfl(r, who, kWave), hh = __shfl(held, who, kWave), base = __shfl(at, who, kWave);
-    int found = 0;
-    for (int j0 = 0; j0 < hh; j0 += kWave) {
-      const int page = j0 + lane < hh ? a.table[rr * a.table_ld + j0 + lane] : -1;
-      const uint64_t ok = __ballot(real_page(a, page));
-      if (real_page(a, page)) put(base + found + __popcll(ok & ((1ull << lane) - 1)), page);
-      found += __popcll(ok);
+  uint64_t todo = __ballot(r < a.n_seqs && held > 0 && a.fresh[r] < 0);
+  int count = 0, found = 0, j0 = 0;
+  while (todo) {
+    int page[FLIGHT], who[FLIGHT];
+    bool last[FLIGHT];
+#pragma unroll
+    for (int i = 0; i < FLIGHT; ++i) {
+      who[i] = todo ? __ffsll(static_cast<unsigned long long>(todo)) - 1 : -1;
+      page[i] = -1;
+      last[i] = false;
+      if (who[i] < 0) continue;
+      const int rr = __builtin_amdgcn_readlane(r, who[i]), hh = __builtin_amdgcn_readlane(held, who[i]);
+      if (j0 + lane < hh) page[i] = a.table[rr * a.table_ld + j0 + lane];
+      j0 += kWave;
+      if (j0 >= hh) {
+        last[i] = true;
+        todo &= todo - 1;
+        j0 = 0;
+      }
     }
-    if (lane == who) count = found;
+#pragma unroll
+    for (int i = 0; i < FLIGHT; ++i) {
+      if (who[i] < 0) continue;
+      const uint64_t ok = __ballot(real_page(a, page[i]));
+      if (real_page(a, page[i])) put(__builtin_amdgcn_readlane(at, who[i]) + found + __popcll(ok & ((1ull << lane) - 1)), page[i]);
+      found += __popcll(ok);
+      if (last[i]) {
+        if (lane == who[i]) count = found;
+        found = 0;
+      }
+    }
   }
   return count;
 }
 // Pages taken: each growing request's first by its own thread (a decode step takes one or none), the others by whole
-// waves.  get(k): the page k places below the top of the stack; keep(k, page).
-template <class Get, class Keep>
-__device__ __forceinline__ void take_pages(const PlanArgs& a, int r, int held, uint32_t take, uint32_t before, Get&& get, Keep&& keep) {
+// waves.  get(k): the page k places below the top of the stack.
+template <class Get>
+__device__ __forceinline__ void take_pages(const PlanArgs& a, int r, int held, uint32_t take, uint32_t before, Get&& get) {
   const int lane = threadIdx.x & (kWave - 1);
-  if (take > 0) {
-    const int page = get(static_cast<int>(before));
-    a.table[r * a.table_ld + held] = page;
-    keep(static_cast<int>(before), page);
-  }
+  if (take > 0) a.table[r * a.table_ld + held] = get(static_cast<int>(before));
   for (uint64_t todo = __ballot(take > 1); todo; todo &= todo - 1) {
     const int who = __ffsll(static_cast<unsigned long long>(todo)) - 1;
     const int rr = __shfl(r, who, kWave), h = __shfl(held, who, kWave), n = __shfl(static_cast<int>(take), who, kWave);
     const int k0 = __shfl(static_cast<int>(before), who, kWave);
-    for (int j = 1 + lane; j < n; j += kWave) {
-      const int page = get(k0 + j);
-      a.table[rr * a.table_ld + h + j] = page;
-      keep(k0 + j, page);
-    }
+    for (int j = 1 + lane; j < n; j += kWave) a.table[rr * a.table_ld + h + j] = get(k0 + j);
   }
 }
 // Whether the step fits, and what does not: the same for every thread.
@@ -190,7 +202,7 @@ __global__ __launch_bounds__(kPlanThreads) void page_plan_kernel(PlanArgs a) {
     const int x = r < a.n_seqs ? a.fresh[r] : 0;
     const Three before = scan_block(s.v, &carry, &part);
     if (v.fits)
-      take_pages(a, r, s.held, s.v.take, before.take, [&](int k) { return a.free_list[static_cast<int>(v.n1) - 1 - k]; }, count_only);
+      take_pages(a, r, s.held, s.v.take, before.take, [&](int k) { return a.free_list[static_cast<int>(v.n1) - 1 - k]; });
     if (r >= a.n_seqs) continue;
     a.row_start[r] = v.fits ? static_cast<int>(before.rows) : 0;
     a.kv_len[r] = !v.fits ? s.cached : x < 0 ? 0 : s.cached + static_cast<int>(s.v.rows);
@@ -200,7 +212,7 @@ __global__ __launch_bounds__(kPlanThreads) void page_plan_kernel(PlanArgs a) {
 // One request to a thread.  The sums are formed once; given pages, taken pages and the requests' starts are kept in LDS
 // too, so that a step waits for memory four times (lengths, ended requests' pages, free pages, the table) and for
 // none of its own stores.
-constexpr int kPlanKept = 2048;  // given and taken pages kept in LDS; beyond, the stores are waited for
+constexpr int kPlanKept = 4096;  // given and taken pages kept in LDS; beyond, the stores are waited for
 
 template <int THREADS, bool FILL>
 __global__ __launch_bounds__(THREADS) void page_plan_once_kernel(PlanArgs a) {
@@ -231,22 +243,24 @@ __global__ __launch_bounds__(THREADS) void page_plan_once_kernel(PlanArgs a) {
   if (t == 0) start_s[a.n_seqs] = v.fits ? static_cast<int>(total.rows) : 0;
   if (kept) lds_barrier();
   else __syncthreads();
-  if (v.fits)
-    take_pages(a, t, s.held, s.v.take, before.take,
-               [&](int k) {
-                 const int at = static_cast<int>(v.n1) - 1 - k;
-                 return kept && at >= n0 ? given_s[at - n0] : a.free_list[at];
-               },
-               [&](int k, int page) {
-                 if (k < kPlanKept) taken_s[k] = page;
-               });
+  auto top = [&](int k) {  // the page k places below the top of the stack
+    const int at = static_cast<int>(v.n1) - 1 - k;
+    return kept && at >= n0 ? given_s[at - n0] : a.free_list[at];
+  };
+  if (kept) {  // every page at once, then the table from LDS
+    if (v.fits)
+      for (int k = t; k < static_cast<int>(total.take); k += THREADS) taken_s[k] = top(k);
+    lds_barrier();
+    if (v.fits) take_pages(a, t, s.held, s.v.take, before.take, [&](int k) { return taken_s[k]; });
+  } else if (v.fits) {
+    take_pages(a, t, s.held, s.v.take, before.take, top);
+  }
   if (t < a.n_seqs) {
     a.row_start[t] = v.fits ? static_cast<int>(before.rows) : 0;
     a.kv_len[t] = !v.fits ? s.cached : x < 0 ? 0 : s.cached + static_cast<int>(s.v.rows);
   }
   if constexpr (FILL) {
-    if (kept) lds_barrier();
-    else __syncthreads();
+    if (!kept) __syncthreads();  // the table's new pages
     const int rows = v.fits ? static_cast<int>(total.rows) : 0;
     for (int i = t; i < a.max_rows; i += THREADS) {
       int p = 0;

@@ -122,10 +122,11 @@ def same_plan(got, want):
 
 
 # requests on both sides of one pass of the workgroup (1024) and of what it keeps in LDS (4096); rows on both sides
-# of what it fills by itself (4096)
+# of what it fills by itself (4096); pages given or taken on both sides of what it keeps (4096)
 @pytest.mark.parametrize("n,page,ctx,most", [(1, 16, 0, 1), (1, 1, 5, 3), (64, 16, 900, 1), (63, 8, 100, 200), (1023, 32, 300, 2),
                                              (1024, 16, 64, 1), (1025, 16, 64, 1), (2500, 4, 30, 9), (4096, 16, 20, 1), (4097, 16, 20, 2),
-                                             (700, 32, 4000, 30), (3, 1024, 5000, 3000)])
+                                             (700, 32, 4000, 30), (3, 1024, 5000, 3000),
+                                             (200, 1, 300, 2), (200, 1, 4, 60), (900, 2, 90, 40)])
 @pytest.mark.parametrize("in_place", [False, True])
 def test_plan(hip, n, page, ctx, most, in_place):
     print(f"[case] plan n={n} page={page} ctx={ctx} most={most} in_place={in_place}", flush=True)
