@@ -60,6 +60,9 @@ Split split_over(size_t wgs, size_t want, size_t longest, size_t least, size_t s
 // Positions are split so that the workgroups fill the GPU once (as many as its CUs hold at the kernels' registers): one
 // more than fits costs a second round.  12 x 32k BF16: 5 ranges (480 workgroups of 512) 215 us, 8 (768) 271, 10 (960)
 // 237; 64 requests of 2047 FP16: 3 ranges (768 of 768) 26.8 us, 4 (1024) 32.
+// The tiles kernel's shortest range is 256 positions, 128 after at most 1536, where that leaves workgroups idle.  FP16, us with
+// 256 / 128: 8 requests of 1000 positions (64 dims) 17.5 / 15.6, 200 rows after 200 (128 dims) 22.5 / 19.7, 32 rows after
+// 8000 (128 dims) 34.8 / 44.9, 20 requests of 4000 (64 dims) 31.7 / 34.0.
 PagedPlan plan_paged(size_t H, size_t KV, size_t hd, int qtype, size_t n_seqs, size_t max_rows, size_t max_new, size_t max_kv) {
   PagedPlan p;
   const size_t cus = ctx().cu_count > 0 ? ctx().cu_count : 256;
@@ -82,11 +85,14 @@ PagedPlan plan_paged(size_t H, size_t KV, size_t hd, int qtype, size_t n_seqs, s
   return p;
 }
 
-// Whether packed FP32 and BF16 rows go through the prepared tiles: fewer products, one more launch and pass.  By the
+// Whether packed FP32 and BF16 rows go through the prepared tiles: FP32 rows scaled and split
+// once instead of by every workgroup, BF16 two products for three; one more launch and pass.  By the
 // work, rows times rows of a prompt on average; us from the rows / prepared, 32 heads over 4 of 64 and over 8 of 128:
-//   FP32, 64:   200 rows 15.5 / 15.8, 333 of 9 prompts 11.1 / 14.5, 500 rows 27.8 / 23.9, 1000 of 8 25.6 / 25.6, 2000 rows
-//               111 / 77
-//   FP32, 128:  100 rows 19.1 / 18.0, 500 rows 66.5 / 39.5, 2000 of 20 58 / 49   (80 and 256: ahead from 64 rows)
+//   FP32, 64:   100 rows 11.2 / 12.8, 200 rows 16.0 / 15.3, 333 of 9 prompts 11.5 / 13.8, 500 rows 28.0 / 23.2, 1000 of 8
+//               25.6 / 23.6, 2000 of 20 25.4 / 25.8, 2000 rows 95.3 / 73.0
+//   FP32, 128:  100 rows 18.6 / 16.5, 333 of 9 20.8 / 18.7, 500 rows 60.6 / 37.4, 2000 of 20 54.7 / 40.3
+//   FP32, 80 (12 heads over 4):  64 rows 10.9 / 12.6, 128 rows 15.9 / 15.0, 256 of 4 23.8 / 19.4
+//   FP32, 256 (8 over 4):  64 rows 28.8 / 26.7, 128 rows 41.8 / 33.8
 //   BF16, 64:   1000 rows 30.2 / 32.5, 1500 of 3 37 / 40, 2000 rows 61.5 / 59.1, 6000 of 4 181 / 144, 9000 rows 804 / 623
 //   BF16, 128:  1000 rows 46 / 57, 2000 rows 102 / 105, 3000 rows 188 / 157, 9000 rows 1443 / 1170
 // EF_HIP_PACKED_ATTENTION=rows|prepared takes one or the other (tests).
@@ -97,7 +103,7 @@ bool prepares(size_t hd, int qtype, size_t n_seqs, size_t max_rows) {
     if (std::strcmp(e, "prepared") == 0) return true;
   }
   const double work = static_cast<double>(max_rows) * max_rows / n_seqs;
-  return work >= (qtype == EF_QTYPE_BF16 ? 4194304.0 : hd <= 64 ? 131072.0 : 4096.0);
+  return work >= (qtype == EF_QTYPE_BF16 ? 4194304.0 : hd <= 64 ? 131072.0 : hd <= 128 ? 8192.0 : 4096.0);
 }
 
 size_t prepared_places(size_t hd, int qtype, size_t n_seqs, size_t max_rows) {
