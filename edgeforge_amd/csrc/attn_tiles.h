@@ -6,8 +6,15 @@
 // positions 8 (i / 4) + 4 h + i % 4, pair lane % 32, h = lane / 32).  The k slots of a product may hold
 // positions in any order, so the weights feed O^T += V^T P^T from the registers they were computed in, against
 // V read transposed from LDS (ds_read_b64_tr_b16: 16 lanes read four positions' rows of 16 dims and get four
-// positions of a dim each).  16-bit parts of the queries and the weights keep FP32's accuracy (attn_core.h); FP32
-// keys and values are split into three parts as they are staged.
+// positions of a dim each).  16-bit parts of the queries and the weights keep FP32's accuracy (attn_core.h): two
+// products for FP16 keys and values, three for BF16.  FP32 tiles are scaled by powers of two and split into two
+// FP16 parts (three products), as they are staged or, for packed rows with enough work, by a kernel before.
+//
+// Bound by the matrix cores' rate under load: 9001 packed FP16 rows (508 GFLOP of attention, twice that in
+// products) 884 us, 1150 TFLOP/s of products where a large library product reaches 1187 (matrix units busy 58 to 60% of
+// the cycles, the clock falling from 1.82 to 1.52 GHz over three launches); 6001 FP32 rows 217 us, with the preparation, 8 to 11 in its traces; 500 rows after 8111 positions
+// of FP16 pages 150 us with the join.  Six products of three BF16 parts took 350 us for the 6001 FP32 rows; tiles
+// through registers instead of LDS-DMA 941 us for the 9001 (868 when first changed); sums taken in turn made no difference.
 //
 // Masked positions: scores -inf; rows past the last position or without a page are staged as zeros.  Pairs whose
 // sums come out infinite or NaN are computed again by wave_attend, which reads only what each row sees.
