@@ -222,6 +222,8 @@ struct AttnTask {
   int few_most;  // (row, head) pairs of a KV head up to which a request is the few-rows kernel's, not the tiles kernel's
 };
 
+// Ranges from which on a (row, head) pair's join has a workgroup of its own, not a wave.
+constexpr int kJoinMany = 16;
 // (row, head) pairs of a KV head in a workgroup of the tiles kernel
 constexpr int kTilePairs = 128;
 

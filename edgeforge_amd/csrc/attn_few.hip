@@ -10,7 +10,7 @@ namespace {
 // are many ranges (one request of 30000 positions: 236 of them).  A lane takes 4 dims of every (waves 64 / (hd / 4))th
 // range.  The lengths are not read: the first range's workgroup left their number beside its sums, and the loads of the
 // first ranges do not wait for it (what they read beyond it is not used).
-constexpr int kJoinFirst = 4, kJoinMany = 16;
+constexpr int kJoinFirst = 4;
 
 template <int LANES, bool MANY>  // lanes to a row: 16, 32 or 64; MANY: a workgroup to a row
 __global__ __launch_bounds__(256) void attention_join_kernel(AttnTask t) {

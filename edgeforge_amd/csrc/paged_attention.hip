@@ -160,9 +160,14 @@ int ef_hip_paged_attention(const float* q, size_t ldq, float* out, size_t ldo, s
             "paged_attention: the workspace must have ef_hip_paged_attention_workspace_bytes bytes, at a multiple of 16");
   EFH_CHECK(static_cast<size_t>(p.few_tiles) * p.few_split.splits <= 65535, "paged_attention: too many heads to a KV head");
   // workgroups of a launch: places of tiles and requests, by KV heads and ranges
-  const double groups = (static_cast<double>(b.max_rows) * heads / pool->KV / kTilePairs + 1 + b.n_seqs) * pool->KV * p.tile_split.splits +
-                        static_cast<double>(b.n_seqs) * pool->KV * p.few_tiles * p.few_split.splits;
-  EFH_CHECK(groups < 2147483647.0, "paged_attention: too many requests, rows and heads for one launch");
+  const double tiles = (static_cast<double>(b.max_rows) * heads / pool->KV / kTilePairs + 1 + b.n_seqs) * pool->KV;
+  const double few = static_cast<double>(b.n_seqs) * pool->KV * p.few_tiles * p.few_split.splits;
+  // (the ranges are along x in the launch of both kernels, along y in the tiles kernel's own)
+  EFH_CHECK(!p.tiles || (p.few ? tiles * p.tile_split.splits + few : tiles) <= static_cast<double>(kGridMost),
+            "paged_attention: too many requests, rows and heads for one launch");
+  const size_t ranges = std::max(p.few_split.splits, p.tile_split.splits);
+  EFH_CHECK(ranges <= 1 || b.max_rows * heads <= kGridMost * (ranges > kJoinMany ? 1 : 4),
+            "paged_attention: too many rows and heads for one launch");
   EFH_RC(require_ready());
   if (b.max_rows == 0) return EF_HIP_OK;
   AttnTask t = task_of(a);
@@ -219,7 +224,7 @@ int ef_hip_packed_attention(const float* q, size_t ldq, const void* k, size_t ld
   const size_t need = prepared_bytes(KV, hd, qtype, n_seqs, max_rows);
   EFH_CHECK(need == 0 || (ws != nullptr && ws_bytes >= need && aligned16(ws)),
             "packed_attention: the workspace must have ef_hip_packed_attention_workspace_bytes bytes, at a multiple of 16");
-  EFH_CHECK((static_cast<double>(max_rows) * heads / KV / kTilePairs + 1 + n_seqs) * KV < 2147483647.0,
+  EFH_CHECK((static_cast<double>(max_rows) * heads / KV / kTilePairs + 1 + n_seqs) * KV <= static_cast<double>(kGridMost),
             "packed_attention: too many prompts, rows and heads for one launch");
   EFH_RC(require_ready());
   if (max_rows == 0) return EF_HIP_OK;

@@ -17,6 +17,9 @@ inline size_t pool_stride(const ef_hip_page_pool& p) { return p.page_stride ? p.
 inline int log2_of(size_t pow2) { return __builtin_ctzll(pow2); }
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
+// Workgroups of 256 threads that one launch takes along x: HIP counts the threads in 32 bits.
+constexpr size_t kGridMost = (size_t(1) << 24) - 1;
+
 // The request of row i: the last r with start[r] <= i, for start[0] <= i < start[n] (requests without rows are
 // passed over, as the next one starts at the same row).
 template <class P>

@@ -489,7 +489,7 @@ int ef_hip_rope_append(const float* q, size_t ldq, float* q_out, size_t ldqo, si
   EFH_CHECK((q_out != q || ldqo == ldq) && (k_out != k || ldko == ldk),
             "rope_append: rows turned in place need the same stride on both sides");
   const size_t items = (heads + 2 * pool->KV) * (pool->hd / 8);
-  EFH_CHECK(rows <= 0x7FFFFFFF && rows <= (size_t(0x7FFFFFFF) * 256) / items, "rope_append: too many rows");
+  EFH_CHECK(rows <= 0x7FFFFFFF && rows <= kGridMost * 256 / items, "rope_append: too many rows");
   const AppendArgs a{q, k, v, q_out, k_out, static_cast<long>(ldq), static_cast<long>(ldqo), static_cast<long>(ldk),
                      static_cast<long>(ldko), static_cast<long>(ldv), static_cast<long>(rows), static_cast<int>(heads),
                      static_cast<int>(pool->KV), static_cast<int>(pool->hd), static_cast<int>(n_pos), pos, cos_dev, sin_dev,

@@ -1,0 +1,55 @@
+"""Sizes that one launch cannot take, the workspace of sizes that the call refuses, and ids and slots that a PagedEngine
+has not got: on the CPU, nothing is launched."""
+import ctypes as C
+import os
+import subprocess
+import sys
+
+import numpy as np
+import pytest
+
+from edgeforge_amd import _lib as L
+from edgeforge_amd.model import PagedEngine
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+P = 0x10000
+
+PROGRAM = r"""
+import ctypes as C, sys
+from edgeforge_amd import _lib as L
+P = 0x10000
+lib = L.lib()
+def rc(name, *a):
+    return getattr(lib, name)(*a)
+wrong = []
+def expect(what, want, got):
+    if got != want: wrong.append((what, got, (lib.ef_hip_last_error() or b"").decode()))
+
+# a launch takes fewer than 2^32 threads along x
+pool = L.ef_hip_page_pool(P, P, L.F16, 9, 16, 2, 64, 0)
+def append(rows):
+    return rc("ef_hip_rope_append", P, 256, P, 256, 4, P, 128, None, 0, P, 128, rows, P, P, P, 64, P, C.byref(pool), None)
+items = (4 + 2 * 2) * 8
+most = ((1 << 32) - 256) // items
+expect("append, most rows", L.ESTATE, append(most))
+expect("append, one more block", L.EINVAL, append(most + 8))
+
+def packed(n_seqs):
+    return rc("ef_hip_packed_attention", P, 1024, P, 1024, P, 1024, L.F16, P, 1024, 16, 16, 64, P, n_seqs, 8, 0.125, P, 1 << 50, None)
+expect("packed, most prompts", L.ESTATE, packed((1 << 20) - 8))
+expect("packed, one workgroup more", L.EINVAL, packed(1 << 20))
+pool16 = L.ef_hip_page_pool(P, P, L.F16, 9, 16, 16, 64, 0)
+def paged(n_seqs, rows, max_new, max_kv, pool, heads):
+    b = L.ef_hip_paged_batch(P, P, P, 4, n_seqs, rows, max_new, max_kv)
+    return rc("ef_hip_paged_attention", P, heads * 64, P, heads * 64, heads, C.byref(pool), C.byref(b), 0.125, P, 1 << 60, None)
+expect("decode of the most requests", L.ESTATE, paged(1 << 20, 8, 1, 100, pool16, 16))  # along x, y and z
+expect("chunks of too many", L.EINVAL, paged(1 << 20, 8, 500, 100, pool16, 16))
+expect("two ranges joined, most rows", L.ESTATE, paged(1, (1 << 24) - 1, 1, 200, pool, 4))
+expect("two ranges joined, more", L.EINVAL, paged(1, 1 << 24, 1, 200, pool, 4))
+sys.exit(print(wrong) or (1 if wrong else 0))
+"""
+
+
+def test_launches_too_large_are_refused():
+    r = subprocess.run([sys.executable, "-c", PROGRAM], cwd=ROOT, capture_output=True, text=True)
+    assert r.returncode == 0, r.stdout + r.stderr
