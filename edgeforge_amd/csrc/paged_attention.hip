@@ -125,7 +125,7 @@ extern "C" {
 size_t ef_hip_paged_attention_workspace_bytes(size_t heads, const ef_hip_page_pool* pool, size_t n_seqs, size_t max_rows,
                                               size_t max_new, size_t max_kv) {
   if (check_page_pool(pool, "paged_attention") != EF_HIP_OK || heads < 1 || heads > 65535 || heads % pool->KV != 0 ||
-      n_seqs < 1 || max_rows > (size_t(1) << 30) || max_kv > 0x7FFFFFFF)
+      n_seqs < 1 || n_seqs > (size_t(1) << 20) || max_rows > (size_t(1) << 30) / heads || max_kv > 0x7FFFFFFF)
     return 0;
   return plan_paged(heads, pool->KV, pool->hd, pool->qtype, n_seqs, max_rows, max_new, max_kv).bytes;
 }

@@ -53,3 +53,9 @@ sys.exit(print(wrong) or (1 if wrong else 0))
 def test_launches_too_large_are_refused():
     r = subprocess.run([sys.executable, "-c", PROGRAM], cwd=ROOT, capture_output=True, text=True)
     assert r.returncode == 0, r.stdout + r.stderr
+
+
+@pytest.mark.parametrize("seqs,rows", [(1, 1 << 30), (1, (1 << 28) + 1), ((1 << 20) + 1, 8)])
+def test_workspace_of_sizes_the_call_refuses_is_zero(seqs, rows):
+    pool = L.ef_hip_page_pool(P, P, L.F16, 9, 16, 4, 64, 0)
+    assert L.lib().ef_hip_paged_attention_workspace_bytes(4, C.byref(pool), seqs, rows, 1, 8000) == 0
