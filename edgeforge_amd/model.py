@@ -336,6 +336,8 @@ class PagedEngine:
 
     def release(self, *slots: int) -> None:
         """The slots' pages back to the pool; the slots are free for other requests."""
+        if any(not 0 <= s < self.seqs for s in slots):
+            raise ValueError(f"{slots}: no such slot")
         new = np.zeros(self.seqs, np.int32)
         new[list(slots)] = -1
         self._plan(new)

@@ -59,3 +59,24 @@ def test_launches_too_large_are_refused():
 def test_workspace_of_sizes_the_call_refuses_is_zero(seqs, rows):
     pool = L.ef_hip_page_pool(P, P, L.F16, 9, 16, 4, 64, 0)
     assert L.lib().ef_hip_paged_attention_workspace_bytes(4, C.byref(pool), seqs, rows, 1, 8000) == 0
+
+
+class _Config:
+    V = 100
+
+
+def _engine():
+    """An engine's bookkeeping alone; anything that reaches the device fails the test."""
+    e = object.__new__(PagedEngine)
+    e.cfg, e.seqs, e.rows, e.max_seq, e.lens, e.stream = _Config(), 4, 16, 32, np.zeros(4, np.int32), None
+
+    def launched(*a, **k):
+        raise AssertionError("went on to the device")
+    e._plan = e._workspace = launched
+    return e
+
+
+@pytest.mark.parametrize("slot", [-1, 4, 1 << 40])
+def test_release_of_no_slot_is_refused(slot):
+    with pytest.raises(ValueError, match="no such slot"):
+        _engine().release(slot)
