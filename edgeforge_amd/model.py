@@ -302,7 +302,7 @@ class PagedEngine:
         PagesShort, with nothing changed, when the pages do not suffice (release some, or wait)."""
         slots = sorted(tokens)
         new = np.zeros(self.seqs, np.int32)
-        ids = [np.asarray(tokens[s], np.int32).reshape(-1) for s in slots]
+        ids = [self._ids_of(tokens[s]) for s in slots]
         for s, t in zip(slots, ids):
             if not 0 <= s < self.seqs or t.size == 0:
                 raise ValueError(f"slot {s}: no such slot, or no tokens")
@@ -350,6 +350,7 @@ class PagedEngine:
         different lengths in one pass, without pages)."""
         c, s = self.cfg, self.stream
         out, at = [None] * len(windows), 0
+        windows = [self._ids_of(w) for w in windows]
         lens = [len(w) - 1 for w in windows]
         if any(n < 1 or n > min(self.rows, self.max_seq) for n in lens):
             raise ValueError(f"windows of 2 to {min(self.rows, self.max_seq) + 1} ids")
@@ -358,8 +359,8 @@ class PagedEngine:
             while at + len(group) < len(windows) and n + lens[at + len(group)] <= self.rows and len(group) < self.seqs:
                 n += lens[at + len(group)]
                 group.append(at + len(group))
-            up = {self._ids: np.concatenate([np.asarray(windows[i][:-1], np.int32) for i in group]),
-                  self._last: np.concatenate([np.asarray(windows[i][1:], np.int32) for i in group]),
+            up = {self._ids: np.concatenate([windows[i][:-1] for i in group]),
+                  self._last: np.concatenate([windows[i][1:] for i in group]),
                   self._pos: np.concatenate([np.arange(lens[i], dtype=np.int32) for i in group]),
                   self._slot: np.full(n, -1, np.int64),
                   self._start: np.concatenate([[0], np.cumsum([lens[i] for i in group])]).astype(np.int32)}
@@ -388,6 +389,12 @@ class PagedEngine:
                 r0 += lens[i]
             at += len(group)
         return out
+
+    def _ids_of(self, tokens) -> np.ndarray:
+        t = np.asarray(tokens).reshape(-1)
+        if t.size and (t.dtype.kind not in "iu" or t.min() < 0 or t.max() >= self.cfg.V):
+            raise ValueError(f"token ids are integers in the vocabulary, 0 to {self.cfg.V - 1}")
+        return t.astype(np.int32)
 
     # ---- parts ---------------------------------------------------------------------------------------
     def _plan(self, new: np.ndarray) -> None:

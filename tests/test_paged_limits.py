@@ -80,3 +80,15 @@ def _engine():
 def test_release_of_no_slot_is_refused(slot):
     with pytest.raises(ValueError, match="no such slot"):
         _engine().release(slot)
+
+
+@pytest.mark.parametrize("ids", [[-1], [100], [3, 1 << 33]])
+def test_step_of_ids_outside_the_vocabulary_is_refused(ids):
+    with pytest.raises(ValueError, match="vocabulary"):
+        _engine().step({0: ids})
+
+
+@pytest.mark.parametrize("window", [[1, -1], [100, 2], [1, 2, (1 << 32) + 3]])
+def test_score_of_ids_outside_the_vocabulary_is_refused(window):
+    with pytest.raises(ValueError, match="vocabulary"):
+        _engine().score([[1, 2, 3], window])
