@@ -383,13 +383,14 @@ int ef_hip_rope_append(const float* q_dev, size_t ldq, float* q_out_dev, size_t 
  * n positions, so row i sees positions 0 .. kv_len_dev[r] - n + i:
  *   out = sum_j softmax_j(scale * q . k_j) v_j,  query head h over KV head h / (heads / KV).
  * A page number outside [0, n_pages) is no page: its positions take no part.  A row that sees nothing
- * gets zeros.  Rows behind row_start_dev[n_seqs] stay as they were.  Infinite or NaN keys and values
+ * gets zeros, as one whose scores are all -inf does.  Rows behind row_start_dev[n_seqs] stay as they were.  Infinite or NaN keys and values
  * stay with the rows that see them.  q / out are FP32 rows [..][heads * hd] with strides ldq / ldo.
  * Everything is held in 32 bits or more; results are the same on every call.
  * The bounds are the host's: max_rows rows in q and out, max_new rows of one request, max_kv positions
  * of one request.  max_rows is kept to (rows behind it are neither read nor written); max_new and
  * max_kv choose the kernel and its split, lengths above them are right but slow.
- * ws_dev: ef_hip_paged_attention_workspace_bytes of the same sizes (may be 0: then ws_dev may be NULL). */
+ * ws_dev: ef_hip_paged_attention_workspace_bytes of the same sizes (may be 0: then ws_dev may be NULL); calls
+ * that may run at the same time, those of two captured graphs among them, need one each.  out overlaps no input. */
 typedef struct {
   const int32_t *row_start_dev, *kv_len_dev, *table_dev;
   size_t table_ld, n_seqs, max_rows, max_new, max_kv;
