@@ -58,14 +58,14 @@ __device__ __forceinline__ void attention_few(const AttnTask& t, FewLds<HDP, NT>
 #pragma unroll
     for (int u = 0; u < TILES; ++u) pages[u] = a.kv.table[base + (min(c0 + 16 * u, width) >> sh)];
   }
-  const int first = max(a.row_start[req], 0), n = min(a.row_start[req + 1], a.max_rows) - first;
+  const int first = max(a.row_start[req], 0), next = a.row_start[req + 1], n = min(next, a.max_rows) - first;
   const int kv_len = a.kv_len[req];
   const int kv = static_cast<int>(min(static_cast<long>(kv_len), a.kv.table_ld << a.kv.page_shift));
   if (n <= 0 || static_cast<long>(n) * G > t.few_most) return;
   const int ns = splits_of(kv, t.few_split);
   if (split >= ns) return;
   const int j0 = split * t.few_split.span, j1 = split == t.few_split.splits - 1 ? max(kv, 0) : min(max(kv, 0), j0 + t.few_split.span);
-  const int before = kv_len - n;  // row i sees positions 0 .. before + i
+  const int before = kv_len - (next - first);  // row i sees positions 0 .. before + i; rows cut by max_rows count
   const T *kp = static_cast<const T*>(a.kv.k), *vp = static_cast<const T*>(a.kv.v);
 
   // this lane's dims: K pieces (clamped into the row: the query is zero there), V pieces

@@ -181,7 +181,7 @@ __device__ __forceinline__ void attention_tiles(const AttnTask& t, const Prepare
   if constexpr (PAGED) {
     const int kv_len = a.kv_len[req];
     kv = static_cast<int>(min(static_cast<long>(kv_len), a.kv.table_ld << a.kv.page_shift));
-    before = kv_len - n;
+    before = kv_len - (who.next - first);  // rows cut by max_rows count
     base = req * a.kv.table_ld;
   } else {
     kv = n;

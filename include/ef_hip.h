@@ -387,8 +387,9 @@ int ef_hip_rope_append(const float* q_dev, size_t ldq, float* q_out_dev, size_t 
  * stay with the rows that see them.  q / out are FP32 rows [..][heads * hd] with strides ldq / ldo.
  * Everything is held in 32 bits or more; results are the same on every call.
  * The bounds are the host's: max_rows rows in q and out, max_new rows of one request, max_kv positions
- * of one request.  max_rows is kept to (rows behind it are neither read nor written); max_new and
- * max_kv choose the kernel and its split, lengths above them are right but slow.
+ * of one request.  max_rows is kept to (rows behind it are neither read nor written; those of the same request
+ * before it see what they see without the cut); max_new and max_kv choose the kernel and its split, lengths above
+ * them are right but slow.
  * ws_dev: ef_hip_paged_attention_workspace_bytes of the same sizes (may be 0: then ws_dev may be NULL); calls
  * that may run at the same time, those of two captured graphs among them, need one each.  out overlaps no input. */
 typedef struct {
