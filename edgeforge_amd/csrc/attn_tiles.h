@@ -124,15 +124,49 @@ __device__ __forceinline__ void tile_barrier() {
 
 constexpr int kNoTile = INT32_MIN, kAnyScale = INT32_MAX;
 
-// A tile's exponents from the bits of the largest magnitude of its keys and of its values, and of the smallest among its
-// rows' largest magnitudes (rows of zeros left out).
-__device__ __forceinline__ int2 tile_scales(uint32_t k_most, uint32_t k_least, uint32_t v_most, uint32_t v_least) {
-  const int ek = k_most == 0 ? kAnyScale : (14 + 127 - static_cast<int>(k_most >> 23)) & ~7;
-  const int ev = v_most == 0 ? kAnyScale : (14 + 127 - static_cast<int>(v_most >> 23)) & ~7;
-  const bool marked = k_most >= 0x7F800000u || v_most >= 0x7F800000u || (k_most != 0 && static_cast<int>(k_least >> 23) - 127 + ek < -1) ||
-                      (v_most != 0 && static_cast<int>(v_least >> 23) - 127 + ev < -1);
-  return marked ? int2{kNoTile, kNoTile} : int2{ek, ev};
+// A tile's exponents, and what the largest value of each of its dims has to reach, from the bits of the largest
+// magnitude of its keys and of its values and of the smallest among its rows' largest magnitudes (rows of zeros left
+// out).  Keys are brought to 2^14 .. 2^15 (c2 takes each tile's scale back), values to 2^11 .. 2^15, so that neighbouring tiles
+// mostly share a scale and the sums keep theirs.
+//   What the halves drop of a value is 2^-25 at most or 2^-22 of it: below 2^-24 of (its row's largest) (its dim's largest) /
+//   (the tile's largest) as long as that is 1/2 or more for each row and dim.  The tile's largest is below 2^(M + 1), the rows' are
+//   2^L or more: a dim's largest has to reach 2^(M - L) (all of them scaled).  Dims of zeros are left out.
+struct TileScales {
+  int2 e;
+  float k_dim, v_dim;
+};
+__device__ __forceinline__ TileScales tile_scales(uint32_t k_most, uint32_t k_least, uint32_t v_most, uint32_t v_least) {
+  auto lead = [](uint32_t most, uint32_t least) {  // subnormal rows: the tile is marked
+    return most == 0 ? 0 : least < 0x00800000u ? 15 : static_cast<int>(most >> 23) - static_cast<int>(least >> 23);
+  };
+  const int lk = lead(k_most, k_least), lv = lead(v_most, v_least);
+  const int ek = k_most == 0 ? kAnyScale : 14 + 127 - static_cast<int>(k_most >> 23);
+  const int ev = v_most == 0 ? kAnyScale : (14 + 127 - static_cast<int>(v_most >> 23)) & ~3;
+  const bool marked = k_most >= 0x7F800000u || v_most >= 0x7F800000u || max(lk, lv) > 14;  // 2^15: no dim would reach it
+  return {marked ? int2{kNoTile, kNoTile} : int2{ek, ev}, ldexpf(1.0f, lk - ek), ldexpf(1.0f, lv - ev)};
 }
+
+// A thread's 8 dims of a tile's keys or values, over its rows: which hold something else than zero (the low byte), and which a
+// value that is large enough (the next one).  The words of all threads of the same dims are joined by OR.
+template <class F>
+__device__ __forceinline__ uint32_t dim_flags(float least, F&& largest_of) {
+  uint32_t w = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float most = largest_of(i);
+    w |= (most > 0.0f ? 1u << i : 0u) | (most >= least ? 256u << i : 0u);
+  }
+  return w;
+}
+// The same in short: a bit for each dim whose value in one row is large enough, put behind those of w.
+template <class F>
+__device__ __forceinline__ uint32_t large_dims(uint32_t w, float least, F&& value_of) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) w = __builtin_amdgcn_alignbit(w, __float_as_uint(least - fabsf(value_of(i))), 31);
+  return w;
+}
+// Whether the joined words of keys (low half) and values have a dim that is neither zero nor large enough.
+__device__ __forceinline__ bool dim_too_small(uint32_t w) { return w & ~(w >> 8) & 0x00FF00FFu; }
 
 struct PrepareArgs {
   KvSource kv;
@@ -150,6 +184,8 @@ struct TileLds {
   uint32_t ok[2][Sh::BN / 4];  // a byte per position: whether a page holds it
   int lost;                    // some tile so far had a position without a page
   u4v sizes[2][kTileWaves];    // FP32: each wave's largest and smallest rows of the tile
+  uint32_t large[2][Sh::CHUNKS];  // FP32: the tile's large_dims, and its dim_flags
+  uint32_t dims[Sh::CHUNKS];
 };
 
 // One workgroup: the place `place` of KV head `kvh`, range `split`.
@@ -273,6 +309,14 @@ __device__ __forceinline__ void attention_tiles(const AttnTask& t, const Prepare
   auto measure = [&](int slot) {
     if constexpr (F32) {
       u4v found;
+      if constexpr (PAGED) {  // rows without a page are zeros
+#pragma unroll
+        for (int u = 0; u < UNITS; ++u)
+          if (!(real_rows >> u & 1)) {
+#pragma unroll
+            for (int w = 0; w < WORDS; ++w) kr[u][w] = vr[u][w] = u4v{0, 0, 0, 0};
+          }
+      }
 #pragma unroll
       for (int which = 0; which < 2; ++which) {
         uint32_t most = 0, least = 0;  // least: of the complements of rows that are not zero
@@ -282,7 +326,6 @@ __device__ __forceinline__ void attention_tiles(const AttnTask& t, const Prepare
           uint32_t top = 0;
 #pragma unroll
           for (int i = 0; i < 8; ++i) top = max(top, x[i / 4][i % 4] & 0x7FFFFFFFu);
-          top = real_rows >> u & 1 ? top : 0;
           top = max(top, dpp_self_u<0xB1>(top));
           top = max(top, dpp_self_u<0x4E>(top));
           top = max(top, dpp_self_u<0x141>(top));
@@ -307,18 +350,24 @@ __device__ __forceinline__ void attention_tiles(const AttnTask& t, const Prepare
     for (int i = 0; i < 4; ++i) m[i] = __builtin_amdgcn_readfirstlane(m[i]);
     return tile_scales(m[0], ~m[1], m[2], ~m[3]);
   };
-  auto put = [&](int2 sc) {
+  auto put = [&](const TileScales& sc, int slot) {
     if constexpr (F32) {
+      const int chunk = k_place<CHUNKS>(my_place, my_row);
+      uint32_t large = 0;  // in the first unit's rows: hardly ever less than all of them
 #pragma unroll
-      for (int u = 0; u < UNITS; ++u) {
-        const int r = my_row + u * ROWS, chunk = k_place<CHUNKS>(my_place, my_row);
+      for (int which = 0; which < 2; ++which)
+        large = large_dims(large, which ? sc.v_dim : sc.k_dim, [&](int i) { return __uint_as_float((which ? vr[0] : kr[0])[i / 4][i % 4]); });
+      atomicOr(&lds.large[slot][chunk], large);
 #pragma unroll
-        for (int which = 0; which < 2; ++which) {
+      for (int which = 0; which < 2; ++which) {
+        const int own = which ? sc.e.y : sc.e.x, e = own == kAnyScale ? 0 : own;
+#pragma unroll
+        for (int u = 0; u < UNITS; ++u) {
           const u4v(&x)[WORDS] = which ? vr[u] : kr[u];
-          const int e = which ? sc.y : sc.x;
+          const int r = my_row + u * ROWS;
           float f[8];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) f[i] = real_rows >> u & 1 ? ldexpf(__uint_as_float(x[i / 4][i % 4]), e == kAnyScale ? 0 : e) : 0.0f;
+          for (int i = 0; i < 8; ++i) f[i] = ldexpf(__uint_as_float(x[i / 4][i % 4]), e);
           u4v part[2];
           split8<_Float16>(f, part);
           uint16_t* dst = which ? vs[0] + r * HDP + 8 * v_place<CHUNKS>(chunk, r) : ks[0] + r * HDP + 8 * k_place<CHUNKS>(chunk, r);
@@ -328,7 +377,28 @@ __device__ __forceinline__ void attention_tiles(const AttnTask& t, const Prepare
       }
     }
   };
+  // Whether the tile has a dim too small beside the others: the same for every thread, with a barrier in between where the first
+  // units do not answer it.
+  auto small_dims = [&](const TileScales& sc, int slot) {
+    if constexpr (F32) {
+      if (!__any(lds.large[slot][lane % CHUNKS] != 0xFFFFu)) return false;
+      uint32_t flags = 0;
+#pragma unroll
+      for (int which = 0; which < 2; ++which)
+        flags |= dim_flags(which ? sc.v_dim : sc.k_dim, [&](int i) {
+          float most = 0.0f;
+#pragma unroll
+          for (int u = 0; u < UNITS; ++u) most = fmaxf(most, fabsf(__uint_as_float((which ? vr[u] : kr[u])[i / 4][i % 4])));
+          return most;
+        }) << 16 * which;
+      atomicOr(&lds.dims[k_place<CHUNKS>(my_place, my_row)], flags);
+      tile_barrier();
+      return static_cast<bool>(__any(dim_too_small(lds.dims[lane % CHUNKS])));
+    }
+    return false;
+  };
   if (tid == 0) lost_s = 0;
+  if (F32 && tid < CHUNKS) lds.large[0][tid] = lds.large[1][tid] = lds.dims[tid] = 0;
   __syncthreads();
   // this lane's reads: keys' row col, chunk 2 k + h; values' rows 4 h + lane % 16 / 4, dims 16 (lane / 16 % 2) + 4 (lane % 4)
   const int vq = (lane & 15) / 4, vchunk = 2 * (lane >> 4 & 1) + (lane & 3) / 2;
@@ -383,13 +453,17 @@ __device__ __forceinline__ void attention_tiles(const AttnTask& t, const Prepare
   int o_scale = kAnyScale;  // o is times 2^o_scale (scaled tiles)
   int turn = 0;
   for (int c = j0; c < j1; c += BN) {
+    TileScales scaled{};
     if constexpr (F32) {
       measure(turn);
       tile_barrier();  // the tile before is used, and the sizes are there
-      info = scales(turn);
-      if (info.x != kNoTile) put(info);
+      scaled = scales(turn);
+      info = scaled.e;
+      if (tid < CHUNKS) lds.large[turn ^ 1][tid] = lds.dims[tid] = 0;  // read before that barrier
+      if (info.x != kNoTile) put(scaled, turn);
     }
     tile_barrier();  // the tile is there, and the buffer of the tile before is free
+    if (F32 && info.x != kNoTile && small_dims(scaled, turn)) info = int2{kNoTile, kNoTile};
     const int now = F32 ? 0 : turn, ok_now = turn;
     turn ^= 1;
     const int2 tile_info = info;

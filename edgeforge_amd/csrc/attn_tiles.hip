@@ -5,11 +5,9 @@ namespace efh {
 namespace {
 
 // ---- packed FP32 and BF16 rows as FP16 ---------------------------------------------------------------------
-// A tile of BN rows of one KV head times a power of two that brings its largest value to 2^7 .. 2^15 (its exponent a
-// multiple of 8, so that neighbouring tiles mostly share it): FP32 as two planes, the rounded half and what it left,
-// BF16 as one.  A half of a value x below 2^-14 is off by up to 2^-25: below 2^-24 of its row's largest value as long as
-// that is at least 1/2.  Tiles with a row that is smaller (and not zero), or with infinities or NaN, are marked; the
-// attention kernel takes them from the rows themselves.  Three products (high high, high low, low high) serve
+// A tile of BN rows of one KV head times a power of two (tile_scales): FP32 as two planes, the rounded half and what it
+// left, BF16 as one.  Tiles with a row or a dim too small for that beside the others, or with infinities or NaN, are marked;
+// the attention kernel takes them from the rows themselves.  Three products (high high, high low, low high) serve
 // FP32, two serve BF16, where its rows as they are take three.  The tile is written
 // as the kernel's LDS holds it: planes of K, planes of V.
 // Read and written once, in one pass: bound by memory and the launch (6001 rows of 4 heads of 64, 12 + 12 MB: 8 to 11 us).
@@ -17,7 +15,7 @@ template <class T, int HDP>
 __global__ __launch_bounds__(kTileThreads) void attention_prepare_kernel(PrepareArgs a) {
   using Sh = TileShape<T, HDP, kPrepared>;
   constexpr int BN = Sh::BN, CHUNKS = Sh::CHUNKS, UNITS = Sh::UNITS, PLANES = Sh::PLANES, PLANE = Sh::PLANE, ROWS = kTileThreads / CHUNKS;
-  __shared__ uint32_t most_s[2], least_s[2];
+  __shared__ uint32_t most_s[2], least_s[2], dims_s[CHUNKS];
   const int tid = threadIdx.x, kvh = blockIdx.y, chunk = tid % CHUNKS, my_row = tid / CHUNKS;
   const long place = blockIdx.x;
   const Found who = find_request(a.row_start, a.n_seqs, 1, BN, place);
@@ -28,6 +26,7 @@ __global__ __launch_bounds__(kTileThreads) void attention_prepare_kernel(Prepare
     most_s[tid] = 0;
     least_s[tid] = 0xFFFFFFFFu;
   }
+  if (tid < CHUNKS) dims_s[tid] = 0;
   float x[2][UNITS][8];
 #pragma unroll
   for (int kv = 0; kv < 2; ++kv)
@@ -64,14 +63,26 @@ __global__ __launch_bounds__(kTileThreads) void attention_prepare_kernel(Prepare
     }
   }
   __syncthreads();
-  const int2 e = tile_scales(most_s[0], least_s[0], most_s[1], least_s[1]);
+  const TileScales sc = tile_scales(most_s[0], least_s[0], most_s[1], least_s[1]);
   const long at = kvh * static_cast<long>(a.places) + place;
-  if (tid == 0) a.info[at] = e;
-  if (e.x == kNoTile) return;
+  uint32_t flags = 0;
+#pragma unroll
+  for (int kv = 0; kv < 2; ++kv)
+    flags |= dim_flags(kv ? sc.v_dim : sc.k_dim, [&](int i) {
+      float most = 0.0f;
+#pragma unroll
+      for (int u = 0; u < UNITS; ++u) most = fmaxf(most, fabsf(x[kv][u][i]));
+      return most;
+    }) << 16 * kv;
+  atomicOr(&dims_s[chunk], flags);
+  __syncthreads();
+  const bool marked = sc.e.x == kNoTile || __any(dim_too_small(dims_s[(tid & (kWave - 1)) % CHUNKS]));
+  if (tid == 0) a.info[at] = marked ? int2{kNoTile, kNoTile} : sc.e;
+  if (marked) return;
   uint16_t* block = a.blocks + at * (2 * PLANES * PLANE);
 #pragma unroll
   for (int kv = 0; kv < 2; ++kv) {
-    const int own = kv ? e.y : e.x, scale = own == kAnyScale ? 0 : own;
+    const int own = kv ? sc.e.y : sc.e.x, scale = own == kAnyScale ? 0 : own;
 #pragma unroll
     for (int u = 0; u < UNITS; ++u) {
       const int r = my_row + u * ROWS;
