@@ -102,28 +102,31 @@ __device__ void wave_attend(const KvSource& src, int g, int hd, long base, const
 // FP32 accuracy from 16-bit products: an FP32 operand is split into 16-bit parts whose sum keeps 22 bits or more, and
 // the parts' products are summed in FP32 by the matrix cores.
 //   FP16 keys and values: 2 parts (11 bits each, both rounded to nearest).  Their small range is met by a power of
-//     two: queries are brought to 2^14 .. 2^15 by one that c2 takes back, and p is formed as 2^7 p (the
-//     offset stays in sub), so that what falls below the smallest half is below 2^-31 of the largest.
+//     two: queries are brought to 2^14 .. 2^15 by one that c2 takes back, and p is formed as 2^13 p (the
+//     offset stays in sub), so that what the smallest half drops, 2^-25, is below 2^-38 of the largest.
 //   BF16: 3 parts (8 bits each, truncated, exact in all 24 bits and FP32's range).
 // FP32 keys and values are brought to FP16 by a power of two for a tile and split into 2 parts (attn_tiles.h), or
 // multiplied as they are (attn_few.h).
+// kSubSlack: a running sub is raised only when a score passes it by this much (in powers of two; the weights then reach 2^8, and
+// 2^15 of a half's 2^16 with FP16's offset): with one pass over many positions a new maximum comes often, a much larger one
+// hardly ever.
 template <class T>
 struct Parts;
 template <>
 struct Parts<float> {
   static constexpr int N = 1;
-  static constexpr float kSubOffset = 0.0f;
+  static constexpr float kSubOffset = 0.0f, kSubSlack = 8.0f;
 };
 template <>
 struct Parts<_Float16> {
   static constexpr int N = 2;
-  static constexpr float kSubOffset = 7.0f;
+  static constexpr float kSubOffset = 13.0f, kSubSlack = 2.0f;
   typedef h8v V;
 };
 template <>
 struct Parts<__bf16> {
   static constexpr int N = 3;
-  static constexpr float kSubOffset = 0.0f;
+  static constexpr float kSubOffset = 0.0f, kSubSlack = 8.0f;
   typedef b8v V;
 };
 
@@ -186,11 +189,6 @@ __device__ __forceinline__ int query_exponent(float top) {
   const int e = static_cast<int>(__float_as_uint(top) >> 23 & 255);
   return top == 0.0f || e == 255 ? 0 : min(141 - e, 127);
 }
-
-// A running sub is raised only when a score passes it by this much (in powers of two; the weights then reach 2^8, and
-// 2^15 with the offset of FP16): with one pass over many positions a new maximum comes often, a much larger one
-// hardly ever.
-constexpr float kSubSlack = 8.0f;
 
 // ---- the split over positions ----------------------------------------------------------------------------
 // A request's positions are cut into `splits` ranges of `span` (the last one takes the rest, whatever the length);

@@ -40,7 +40,7 @@ __device__ __forceinline__ void attention_few(const AttnTask& t, FewLds<HDP, NT>
   constexpr int TILES = F32 ? 1 : 2, KT = 16 * TILES, DP = HDP / 16;
   constexpr int KW = F32 ? HDP / 16 : HDP / 32;  // 16-byte pieces of a key row in a lane
   constexpr int VROWS = 4 * TILES, VW = F32 ? DP / 4 : DP * 2 / 16 + (DP == 4);  // value rows of a lane, 16-byte pieces each (8 bytes for 4 halves)
-  constexpr float OFFSET = F32 ? 0.0f : Parts<T>::kSubOffset;
+  constexpr float OFFSET = Parts<T>::kSubOffset, SLACK = Parts<T>::kSubSlack;
   constexpr int PAIRS = 16 * NT, LDO = HDP + 4;
   auto& o_s = lds.o;
   auto& stat_s = lds.stat;
@@ -277,7 +277,7 @@ __device__ __forceinline__ void attention_few(const AttnTask& t, FewLds<HDP, NT>
           for (int r = 0; r < 4; ++r) cm = fmaxf(cm, sc[nt][u][r]);
         cm = column_max(cm);
         const float high = cm * c2[nt] - OFFSET;
-        if (__any(high > sub[nt] + kSubSlack)) {
+        if (__any(high > sub[nt] + SLACK)) {
           const float to = fmaxf(sub[nt], high);
           const float al = to == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(sub[nt] - to);
           sub[nt] = to;

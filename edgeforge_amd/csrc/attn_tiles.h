@@ -199,7 +199,7 @@ __device__ __forceinline__ void attention_tiles(const AttnTask& t, const Prepare
   constexpr bool PAGED = SRC == kPages, PREPARED = SRC == kPrepared, F32 = Sh::F32 && !PREPARED, SCALED = F32 || PREPARED;
   constexpr int BN = Sh::BN, SUB = BN / 32, PLANES = Sh::PLANES, CHUNKS = Sh::CHUNKS, PLANE = Sh::PLANE, UNITS = Sh::UNITS;
   constexpr int KK = HC / 16, DT = HC / 32, NS = Parts<C>::N;
-  constexpr float OFFSET = Parts<C>::kSubOffset;
+  constexpr float OFFSET = Parts<C>::kSubOffset, SLACK = Parts<C>::kSubSlack;
   auto &ks = lds.ks, &vs = lds.vs;
   auto& ok_s = lds.ok;
   int& lost_s = lds.lost;
@@ -508,7 +508,7 @@ __device__ __forceinline__ void attention_tiles(const AttnTask& t, const Prepare
           const float s = half_sum(((part[0] + part[1]) + (part[2] + part[3])) + ((part[4] + part[5]) + (part[6] + part[7])));
           const bool sees = j < seen;
           const float high = sees ? s * a.c2 - OFFSET : -INFINITY;
-          if (__any(high > sub + kSubSlack)) {
+          if (__any(high > sub + SLACK)) {
             const float up = fmaxf(sub, high), al = up == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(sub - up);
             sub = up;
             l *= al;
@@ -580,7 +580,7 @@ __device__ __forceinline__ void attention_tiles(const AttnTask& t, const Prepare
 #pragma unroll
       for (int i = 0; i < 16; ++i) cm = fmaxf(cm, sc[s][i]);
     const float high = half_max(cm) * c2t - OFFSET;
-    if (__any(high > sub + kSubSlack)) {
+    if (__any(high > sub + SLACK)) {
       const float to = fmaxf(sub, high);
       const float al = to == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(sub - to);
       sub = to;
