@@ -451,6 +451,7 @@ __device__ __forceinline__ void attention_tiles(const AttnTask& t, const Prepare
     for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
   float sub = -INFINITY, l = 0.0f;
   int o_scale = kAnyScale;  // o is times 2^o_scale (scaled tiles)
+  int usual = kAnyScale;    // the first scaled tile's
   int turn = 0;
   for (int c = j0; c < j1; c += BN) {
     TileScales scaled{};
@@ -476,8 +477,10 @@ __device__ __forceinline__ void attention_tiles(const AttnTask& t, const Prepare
     float c2t = c2;
     if constexpr (SCALED) {
       const int ek = __builtin_amdgcn_readfirstlane(tile_info.x), ev = __builtin_amdgcn_readfirstlane(tile_info.y);
-      // scales that differ by more than 2^48 would leave FP32's range in the sums: such a tile is taken from its rows too
-      const bool plain = ek == kNoTile || (o_scale != kAnyScale && ev != kAnyScale && abs(ev - o_scale) > 48);
+      // A tile whose values are 2^12 and more from the others' in size is taken from its rows too: a weight's parts are held to 2^-38 of
+      // the largest, which is 2^-22 of the output at most as long as no value is more than 2^16 times the others.
+      const bool plain = ek == kNoTile || (usual != kAnyScale && ev != kAnyScale && abs(ev - usual) > 12);
+      if (!plain && usual == kAnyScale) usual = ev;
       const int to = plain ? 0 : ev == kAnyScale ? o_scale : ev;
       if (to != o_scale) {
         if (o_scale != kAnyScale) {

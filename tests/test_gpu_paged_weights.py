@@ -86,6 +86,29 @@ def test_packed(hip, prepared, qtype, hd, gap, exact, bits):  # noqa: F811
     _packed(hip, qtype, hd, gap, exact, bits)
 
 
+# A whole tile's values 2^40 times the others', at weights of e^-35 = 2^-50: taken in FP32, so no weight is lost.  The exponent's argument is
+# up to 50: its rounding is half an ulp of 32 .. 64, 32 u, c2's roundings 75 u of it: ln 2 (32 + 75) = 74 u for 20 of the 60 u.
+@pytest.mark.parametrize("qtype", [L.F32, L.BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("first", [0, 64, 128])
+def test_packed_tile_far_larger(hip, prepared, qtype, hd, first):  # noqa: F811
+    print(f"[case] far larger tile {qtype} hd={hd} at {first}", flush=True)
+    p = Packed(hip, hd, qtype, 4, 2, hd, [200])
+    k, v = p.k.double().numpy(), p.v.double().numpy()
+    keys_apart(k, p.q, [(first + 64) % 192 + 1, (first + 64) % 192 + 5], 35.0, True, hd)
+    v[first:first + 64] *= 2.0 ** 40
+    p.k, p.v = torch.from_numpy(k).to(TORCH[qtype]), torch.from_numpy(v).to(TORCH[qtype])
+    q, k, v, got, worst = p.q.astype(np.float64), p.k.double().numpy(), p.v.double().numpy(), p.run().astype(np.float64), 0.0
+    for i in range(p.rows):
+        for h in range(4):
+            s = k[:i + 1, h // 2] @ q[i, h] / np.sqrt(hd)
+            w = np.exp(s - s.max())
+            w /= w.sum()
+            worst = max(worst, (np.abs(got[i, h] - w @ v[:i + 1, h // 2]) / (114 * U * (w @ np.abs(v[:i + 1, h // 2])))).max())
+    print(f"worst component {worst:.2f} of its tolerance", flush=True)
+    assert worst < 1.0
+
+
 def _packed(hip, qtype, hd, gap, exact, bits):
     print(f"[case] weights packed {qtype} hd={hd} gap={gap} {bits}", flush=True)
     p = Packed(hip, hd, qtype, 4, 2, hd, [200])
