@@ -52,12 +52,14 @@ __device__ __forceinline__ void load8(const T* p, float (&x)[8]) {
 }
 
 // What the positions [j0, j1) give one (row, head) pair, by a whole wave: a lane takes every 64th position's
-// score and dims lane + 64 u of the output.  q is in LDS.  The sums join (sub, l, o); only seen positions are
-// read, so infinities and NaN elsewhere do not matter.
+// score and dims lane + 64 u of the output.  q is in LDS.  Only seen positions are read, so infinities and NaN elsewhere do not
+// matter.  Weights are 2^-room of those of the formula, 2^room being more than twice the request's `kv` positions, so that no
+// sum of them times values passes the largest value; sub has the factor.
 template <class T, bool PAGED>
-__device__ void wave_attend(const KvSource& src, int g, int hd, long base, const float* q, float c2, int j0, int j1,
+__device__ void wave_attend(const KvSource& src, int g, int hd, long base, const float* q, float c2, int j0, int j1, int kv,
                             float* sub, double* l, float (&o)[4]) {
-  const int lane = threadIdx.x & (kWave - 1);
+  const int lane = threadIdx.x & (kWave - 1), room = 33 - __clz(max(kv, 1));
+  const float weight = ldexpf(1.0f, -room);
   const T *kp = static_cast<const T*>(src.k), *vp = static_cast<const T*>(src.v);
   for (int c = j0; c < j1; c += kWave) {
     const int j = c + lane;
@@ -82,7 +84,7 @@ __device__ void wave_attend(const KvSource& src, int g, int hd, long base, const
       *sub = top;
     }
     const float from = *sub == -INFINITY ? 0.0f : *sub;
-    const float p = seen ? __builtin_amdgcn_exp2f(fmaf(s, c2, -from)) : 0.0f;
+    const float p = seen ? __builtin_amdgcn_exp2f(fmaf(s, c2, -from)) * weight : 0.0f;
     *l += static_cast<double>(p);
     float oc[4] = {0, 0, 0, 0};  // the chunk's own sum: no chain of additions is longer than 64 or the chunks
     for (uint64_t todo = __ballot(seen); todo; todo &= todo - 1) {
@@ -96,6 +98,7 @@ __device__ void wave_attend(const KvSource& src, int g, int hd, long base, const
 #pragma unroll
     for (int u = 0; u < 4; ++u) o[u] = fmaf(o[u], al, oc[u]);
   }
+  *sub += static_cast<float>(room);
 }
 
 // ---- matrix-core operands ------------------------------------------------------------------------------

@@ -395,7 +395,7 @@ __device__ __forceinline__ void attention_few(const AttnTask& t, FewLds<HDP, NT>
         __builtin_amdgcn_wave_barrier();
         float sb = -INFINITY, ov[4] = {0, 0, 0, 0};
         double ll = 0.0;
-        wave_attend<T, true>(a.kv, kvh, hd, base, qs, a.c2, j0, min(j1, min(before + row + 1, kv)), &sb, &ll, ov);
+        wave_attend<T, true>(a.kv, kvh, hd, base, qs, a.c2, j0, min(j1, min(before + row + 1, kv)), kv, &sb, &ll, ov);
         ll = wave_sum_d_dpp(ll);
         long out_row, part_row;
         place_of(pair, &out_row, &part_row);

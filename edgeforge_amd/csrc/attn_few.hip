@@ -11,6 +11,8 @@ namespace {
 // range.  The lengths are not read: the first range's workgroup left their number beside its sums, and the loads of the
 // first ranges do not wait for it (what they read beyond it is not used).
 constexpr int kJoinFirst = 4;
+// Of every range's weight, so that up to 1024 sums near FP32's largest do not pass it together.
+constexpr float kJoinRoom = 0x1p-12f;
 
 template <int LANES, bool MANY>  // lanes to a row: 16, 32 or 64; MANY: a workgroup to a row
 __global__ __launch_bounds__(256) void attention_join_kernel(AttnTask t) {
@@ -42,7 +44,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttnTask t) {
   };
   for (int s0 = 0; s0 < ns; s0 += kWave) {
     if (s0 > 0) st = t.stat[min(s0 + lane, ns - 1) * step + at];
-    const float w = s0 + lane < ns && st[0] != -INFINITY ? __builtin_amdgcn_exp2f(st[0] - top) : 0.0f;
+    const float w = s0 + lane < ns && st[0] != -INFINITY ? __builtin_amdgcn_exp2f(st[0] - top) * kJoinRoom : 0.0f;
     if (s0 + lane < ns) l = fmaf(st[1], w, l);
     const int end = min(ns - s0, kWave);  // this round's ranges; the trip counts are the same for every group
     for (int b = 0; b < end; b += kJoinFirst * GROUPS) {

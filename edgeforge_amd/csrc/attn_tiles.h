@@ -676,7 +676,7 @@ __device__ __forceinline__ void attention_tiles(const AttnTask& t, const Prepare
     __builtin_amdgcn_wave_barrier();
     float sb = -INFINITY, ov[4] = {0, 0, 0, 0};
     double ll = 0.0;
-    wave_attend<T, PAGED>(a.kv, kvh, hd, base, qs, a.c2, j0, lim, &sb, &ll, ov);
+    wave_attend<T, PAGED>(a.kv, kvh, hd, base, qs, a.c2, j0, lim, kv, &sb, &ll, ov);
     ll = wave_sum_d_dpp(ll);
     const float inv = ll == 0.0 ? 0.0f : static_cast<float>(1.0 / ll);
     const long to = direct ? static_cast<long>(first + rr) * a.ldo + static_cast<long>(hh) * hd
