@@ -239,6 +239,9 @@ class Engine:
             pass
 
 
+MOST_ROWS = 65535  # rows that one product (and ef_hip_rows_f32) takes
+
+
 class PagesShort(RuntimeError):
     """A step needs more free pages than there are; nothing was changed."""
 
@@ -257,11 +260,15 @@ class PagedEngine:
                  kv_type: int = EL.F32, stream=None):
         """model: a DeviceModel or an EfqModel (which has to outlive this).  rows: new tokens of one step;
         max_seq: positions of one request."""
-        H.init()
         self.model, self.cfg, self.stream = model, model.cfg, stream
         c = self.cfg
-        if c.hd % 8:
-            raise ValueError("paged attention needs a head size that is a multiple of 8")
+        if c.hd % 8 or not 8 <= c.hd <= 256:
+            raise ValueError("paged attention needs a head size that is a multiple of 8 up to 256")
+        if not 1 <= page_size <= 1024 or page_size & (page_size - 1):
+            raise ValueError("page_size must be a power of two up to 1024")
+        if pages < 1:
+            raise ValueError("pages must be at least 1")
+        H.init()
         self.seqs, self.rows, self.page_size, self.pages = seqs, rows, page_size, pages
         self.max_seq = min(max_seq or c.max_pos, c.max_pos)
         self.table_ld = -(-self.max_seq // page_size)
@@ -299,7 +306,8 @@ class PagedEngine:
     # ---- one step -------------------------------------------------------------------------------------
     def step(self, tokens: dict) -> list[int]:
         """tokens: {slot: new ids}.  Runs them all; returns the slots in the order of `logits`' rows.  Raises
-        PagesShort, with nothing changed, when the pages do not suffice (release some, or wait)."""
+        PagesShort, with nothing changed, when the pages do not suffice (release some, or wait).  A step that
+        raises anything else leaves the requests as they were before it, too."""
         slots = sorted(tokens)
         new = np.zeros(self.seqs, np.int32)
         ids = [self._ids_of(tokens[s]) for s in slots]
@@ -312,15 +320,13 @@ class PagedEngine:
         n = int(new.sum())
         if n == 0:
             return []
-        if n > self.rows:
-            raise ValueError(f"{n} new tokens, {self.rows} rows")
-        self._plan(new)
-        c, s = self.cfg, self.stream
+        if n > min(self.rows, MOST_ROWS):
+            raise ValueError(f"{n} new tokens, {min(self.rows, MOST_ROWS)} rows")
+        c, s, lens = self.cfg, self.stream, self.lens
+        max_new, max_kv = int(new.max()), int((lens + new).max())
+        self._workspace(H.paged_attention_workspace_bytes(c.H, self.pools[0], self.seqs, n, max_new, max_kv))
         flat = np.concatenate(ids)
         EL.call("ef_hip_memcpy_h2d", self._ids.ptr, flat.ctypes.data, flat.nbytes, H._s(s))
-        max_new, max_kv = int(new.max()), int(self.lens.max())
-        need = H.paged_attention_workspace_bytes(c.H, self.pools[0], self.seqs, n, max_new, max_kv)
-        self._workspace(need)
 
         def attend(l):
             b = self._qkv.ptr
@@ -329,9 +335,13 @@ class PagedEngine:
             H.paged_attention(b, self.width, self._ctx, c.D, c.H, self.pools[l], self._table, self.table_ld, self._start, self._len,
                               self.seqs, n, max_new, max_kv, self._scale, ws=self._ws, stream=s)
 
-        self._layers_of(n, attend)
-        last = np.cumsum([t.size for t in ids]).astype(np.int32) - 1
-        self._head_of(last, self.logits)
+        try:
+            self._plan(new)
+            self._layers_of(n, attend)
+            self._head_of(np.cumsum([t.size for t in ids]).astype(np.int32) - 1, self.logits)
+        except BaseException:
+            self._take_back(lens)
+            raise
         return slots
 
     def release(self, *slots: int) -> None:
@@ -352,11 +362,12 @@ class PagedEngine:
         out, at = [None] * len(windows), 0
         windows = [self._ids_of(w) for w in windows]
         lens = [len(w) - 1 for w in windows]
-        if any(n < 1 or n > min(self.rows, self.max_seq) for n in lens):
-            raise ValueError(f"windows of 2 to {min(self.rows, self.max_seq) + 1} ids")
+        rows = min(self.rows, MOST_ROWS)
+        if any(n < 1 or n > min(rows, self.max_seq) for n in lens):
+            raise ValueError(f"windows of 2 to {min(rows, self.max_seq) + 1} ids")
         while at < len(windows):  # as many windows as fit the rows
             group, n = [], 0
-            while at + len(group) < len(windows) and n + lens[at + len(group)] <= self.rows and len(group) < self.seqs:
+            while at + len(group) < len(windows) and n + lens[at + len(group)] <= rows and len(group) < self.seqs:
                 n += lens[at + len(group)]
                 group.append(at + len(group))
             up = {self._ids: np.concatenate([windows[i][:-1] for i in group]),
@@ -408,6 +419,14 @@ class PagedEngine:
         if status.any():
             raise RuntimeError(f"page plan refused: {status.tolist()}")
         self.lens = np.where(new < 0, 0, self.lens + new).astype(np.int32)
+
+    def _take_back(self, lens: np.ndarray) -> None:
+        """The lengths and free pages of before a step, which only takes pages: the free ones' list still holds
+        them above its count, and what the table has behind a request's length is not read."""
+        s = self.stream
+        self.lens = lens
+        self._len.upload(lens, s)
+        self._n_free.upload(np.array([self.pages - int((-(-lens // self.page_size)).sum())], np.int32), s)
 
     def _workspace(self, need: int) -> None:
         if need and (self._ws is None or self._ws.nbytes < need):
