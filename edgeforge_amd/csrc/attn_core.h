@@ -223,6 +223,8 @@ struct AttnTask {
   int few_most;  // (row, head) pairs of a KV head up to which a request is the few-rows kernel's, not the tiles kernel's
 };
 
+// Positions of a request: the kernels count two steps (of 128 positions at most) past the last in 32 bits.
+constexpr size_t kMostPositions = (size_t(1) << 31) - 1024;
 // Ranges from which on a (row, head) pair's join has a workgroup of its own, not a wave.
 constexpr int kJoinMany = 16;
 // (row, head) pairs of a KV head in a workgroup of the tiles kernel

@@ -136,8 +136,8 @@ int ef_hip_paged_attention(const float* q, size_t ldq, float* out, size_t ldo, s
   EFH_CHECK(batch != nullptr, "paged_attention: null batch");
   const ef_hip_paged_batch& b = *batch;
   EFH_CHECK(b.kv_len_dev && b.table_dev, "paged_attention: null pointer");
-  EFH_CHECK(b.table_ld >= 1 && b.table_ld <= size_t(0x7FFFFFFF) / pool->page_size,
-            "paged_attention: table_ld must be at least 1, with a request's positions below 2^31");
+  EFH_CHECK(b.table_ld >= 1 && b.table_ld <= kMostPositions / pool->page_size,
+            "paged_attention: table_ld must be at least 1, with at most 2^31 - 1024 positions of a request");
   RowsArgs a{};
   a.q = q;
   a.out = out;

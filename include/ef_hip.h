@@ -386,6 +386,7 @@ int ef_hip_rope_append(const float* q_dev, size_t ldq, float* q_out_dev, size_t 
  * gets zeros, as one whose scores are all -inf does.  Rows behind row_start_dev[n_seqs] stay as they were.  Infinite or NaN keys and values
  * stay with the rows that see them.  q / out are FP32 rows [..][heads * hd] with strides ldq / ldo.
  * Everything is held in 32 bits or more; results are the same on every call.
+ * table_ld pages hold at most 2^31 - 1024 positions.
  * The bounds are the host's: max_rows rows in q and out, max_new rows of one request, max_kv positions
  * of one request.  max_rows is kept to (rows behind it are neither read nor written; those of the same request
  * before it see what they see without the cut); max_new and max_kv choose the kernel and its split, lengths above
