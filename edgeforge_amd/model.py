@@ -253,7 +253,9 @@ class PagedEngine:
 
     `seqs` slots hold one request each; step() takes the new tokens of any of them, release() gives a
     slot's pages back.  After a step, `logits` holds row i's logits [V] on the device for the i-th slot
-    that got tokens (in order of slots): hip.sample and hip.argmax take it from there.  `kv_type` is what
+    that got tokens (in order of slots): hip.sample and hip.argmax take it from there.  step() returns without
+    waiting: what reads `logits` runs on the same `stream` (`stream=` of those calls, `logits.numpy(stream)`) or
+    waits for it.  score() takes `logits` for its own.  `kv_type` is what
     the pages hold (F32 as the engine's cache, F16 or BF16 for half the memory and traffic)."""
 
     def __init__(self, model, pages: int, page_size: int = 16, seqs: int = 64, rows: int = 512, max_seq: int | None = None,
