@@ -62,7 +62,7 @@ __device__ __forceinline__ Found find_request(const int32_t* row_start, int n_se
     const int step = (len + kWave - 1) / kWave, i = lane * step;
     const int start = row_start[min(lo + i, n_seqs)];
     const uint64_t below = __ballot(i < len && place_of(start, lo + i, f, d) <= place);
-    const int at = max(__popcll(below) - 1, 0);
+    const int at = last_lane(below);  // places in front of the first request's: a negative tile of that one
     if (step == 1) {
       const int req = __builtin_amdgcn_readfirstlane(lo + at);
       Found r{req, __builtin_amdgcn_readlane(start, at), 0, 0};

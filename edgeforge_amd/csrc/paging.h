@@ -33,6 +33,10 @@ __host__ __device__ __forceinline__ int request_of(P start, int n, int i) {
   return lo;
 }
 
+// The last lane of a ballot whose lanes are set from the first one on; 0 where none is.  (Not max(__popcll(lanes) - 1, 0): of an
+// unsigned and a signed value that is a double's maximum, 2^32 - 1 for no lane.)
+__host__ __device__ __forceinline__ int last_lane(uint64_t lanes) { return lanes ? 63 - __builtin_clzll(lanes) : 0; }
+
 // Where keys and values come from: pages (table != nullptr) or packed rows.
 struct KvSource {
   const void *k, *v;
