@@ -23,7 +23,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttnTask t) {
   const long at = MANY ? static_cast<long>(blockIdx.x) : static_cast<long>(blockIdx.x) * 4 + wave, step = static_cast<long>(a.max_rows) * a.H;
   const int group = (MANY ? wave * (kWave / LANES) : 0) + lane / LANES, d = 4 * (lane % LANES);
   const int most = max(t.few_split.splits, t.tile_split.splits);
-  const long rows = min(a.row_start[a.n_seqs], a.max_rows);
+  const long before = max(a.row_start[0], 0), rows = min(a.row_start[a.n_seqs], a.max_rows);
   if (at >= step) return;
   const bool in = d < a.hd;
   const float* part = t.part + at * a.hd + (in ? d : 0);
@@ -32,7 +32,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttnTask t) {
 #pragma unroll
   for (int i = 0; i < kJoinFirst; ++i) first[i] = *reinterpret_cast<const f4v*>(part + min(group + i * GROUPS, most - 1) * step * a.hd);
   f2v st = t.stat[min(lane, most - 1) * step + at];
-  if (at >= rows * a.H || ns <= 1) return;
+  if (at < before * a.H || at >= rows * a.H || ns <= 1) return;  // rows of no request have no number either
   float top = lane < ns ? st[0] : -INFINITY;
   for (int s = lane + kWave; s < ns; s += kWave) top = fmaxf(top, t.stat[s * step + at][0]);
   top = wave_max_dpp(top);

@@ -383,7 +383,8 @@ int ef_hip_rope_append(const float* q_dev, size_t ldq, float* q_out_dev, size_t 
  * n positions, so row i sees positions 0 .. kv_len_dev[r] - n + i:
  *   out = sum_j softmax_j(scale * q . k_j) v_j,  query head h over KV head h / (heads / KV).
  * A page number outside [0, n_pages) is no page: its positions take no part.  A row that sees nothing
- * gets zeros, as one whose scores are all -inf does.  Rows behind row_start_dev[n_seqs] stay as they were.  Infinite or NaN keys and values
+ * gets zeros, as one whose scores are all -inf does.  Rows in front of row_start_dev[0] (some of a
+ * batch's requests, by pointers into the plan) and behind row_start_dev[n_seqs] stay as they were.  Infinite or NaN keys and values
  * stay with the rows that see them.  q / out are FP32 rows [..][heads * hd] with strides ldq / ldo.
  * Everything is held in 32 bits or more; results are the same on every call.
  * table_ld pages hold at most 2^31 - 1024 positions.
