@@ -14,8 +14,8 @@ pytestmark = pytest.mark.gpu
                                              ([100, 90], [300, 777], 131), ([100, 1, 60], [300, 77, 200], 103), ([100, 1, 60], [300, 77, 2000], 140),
                                              ([200], [900], 3), ([40, 3], [40, 3], 41)],
                          ids=["decode", "few", "few_one", "tiles", "mixed_few_left", "mixed", "tiles_three_left", "prompts"])
-@pytest.mark.parametrize("hd", [64, 128])
-def test_rows_before_the_cut(hip, qtype, new, kv, max_rows, hd):
+def test_rows_before_the_cut(hip, qtype, new, kv, max_rows):
+    hd = 64 if len(new) == 3 else 128
     print(f"[case] cut {qtype} hd={hd} {new} {kv} at {max_rows}", flush=True)
     p = Paged(hip, hd + max_rows, qtype, 8, 2, hd, 16, new, kv)
     H, ld = p.H, p.H * hd

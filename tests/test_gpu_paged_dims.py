@@ -19,8 +19,8 @@ from tests.test_gpu_paged import TORCH, U, Packed, Paged, prepared  # noqa: F401
 pytestmark = pytest.mark.gpu
 
 # 2 to the power of: value dims, value rows, one key dim (the queries are zero there), other key dims (queries the other way)
-HOW = {"v_dims_9": (9, 0, 0, 0), "v_dims_16": (16, 0, 0, 0), "v_dims_24": (24, 0, 0, 0), "v_dims_40": (40, 0, 0, 0), "v_both_8": (8, 8, 0, 0),
-       "v_both_12": (12, 12, 0, 0), "k_dim_9": (0, 0, 9, 0), "k_dim_14": (0, 0, 14, 0), "k_dim_20": (0, 0, 20, 0), "k_dim_30": (0, 0, 30, 0),
+HOW = {"v_dims_9": (9, 0, 0, 0), "v_dims_16": (16, 0, 0, 0), "v_dims_40": (40, 0, 0, 0), "v_both_12": (12, 12, 0, 0), "k_dim_14": (0, 0, 14, 0),
+       "k_dim_30": (0, 0, 30, 0),
        "k_dims": (0, 0, 0, 12), "zero_dims": (3, 0, 0, 0), "late_dims": (3, 0, 0, 0), "late_small_dims": (30, 0, 0, 0)}
 
 
@@ -60,7 +60,7 @@ def component_check(got, q, k, v, rc, scale, seen_of, what):
 
 
 @pytest.mark.parametrize("qtype", [L.F32, L.BF16], ids=["f32", "bf16"])
-@pytest.mark.parametrize("hd", [64, 96, 128, 256])
+@pytest.mark.parametrize("hd", [64, 256])
 @pytest.mark.parametrize("how", HOW)
 def test_packed_dims(hip, prepared, qtype, hd, how):  # noqa: F811
     print(f"[case] dims packed {'prepared' if prepared else 'rows'} {qtype} hd={hd} {how}", flush=True)
@@ -73,10 +73,10 @@ def test_packed_dims(hip, prepared, qtype, hd, how):  # noqa: F811
     component_check(got, p.q.astype(np.float64), p.k.double().numpy(), p.v.double().numpy(), rc, 1.0 / np.sqrt(hd), lambda i: i + 1, how)
 
 
-@pytest.mark.parametrize("hd", [64, 96, 128, 256])
+@pytest.mark.parametrize("hd,new", [(96, [90]), (128, [90]), (64, [2])], ids=["96-chunk", "128-chunk", "64-few"])
 @pytest.mark.parametrize("how", HOW)
-@pytest.mark.parametrize("new,kv", [([90], [230]), ([2], [230])], ids=["chunk", "few"])
-def test_paged_dims(hip, hd, how, new, kv):
+def test_paged_dims(hip, hd, how, new):
+    kv = [230]
     print(f"[case] dims paged hd={hd} {how} {new}", flush=True)
     p = Paged(hip, hd, L.F32, 2, 1, hd, 16, new, kv)
     rc, kf, qf = factors(how, kv[0], hd)

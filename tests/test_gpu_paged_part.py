@@ -18,8 +18,7 @@ class At:
 @pytest.mark.parametrize("new,kv", [([1, 1, 1, 1], [900, 700, 1200, 5]), ([3, 4, 2, 5], [900, 700, 1200, 77]), ([90, 70, 100, 30], [900, 700, 1200, 77]),
                                     ([1, 90, 1, 3], [900, 700, 1200, 77]), ([1, 1, 1, 1], [900, 30000, 100, 5])],
                          ids=["decode", "few", "tiles", "mixed", "many_ranges"])
-@pytest.mark.parametrize("a,b", [(1, 3), (2, 4), (1, 2)])
-@pytest.mark.parametrize("fill", [0x02, 0xFF])
+@pytest.mark.parametrize("a,b,fill", [(1, 3, 0x02), (2, 4, 0x02), (1, 2, 0xFF)])
 def test_requests_a_to_b(hip, qtype, new, kv, a, b, fill):
     print(f"[case] part {qtype} {new} {kv} {a}:{b} fill={fill}", flush=True)
     p = Paged(hip, 33, qtype, 8, 2, 64, 16, new, kv)
