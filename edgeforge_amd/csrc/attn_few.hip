@@ -87,8 +87,15 @@ void run_join(const AttnTask& t, hipStream_t s) {
   else attention_join_kernel<LANES, false><<<static_cast<unsigned>((pairs + 3) / 4), 256, 0, s>>>(t);
 }
 
+// Workgroups of a CU at the kernel's registers: narrow pages need more of them, but 16 pairs of FP32 heads of 128 still fit twice
+// (16 requests of 2000, pages of 8: 45.8 us; once 59.6).
 template <class T, int HDP, int NT, bool WIDE>
-__global__ __launch_bounds__(kFewWaves * kWave, HDP == 256 ? 1 : (HDP == 64 && NT == 1 ? 3 : 2) - !WIDE) void attention_few_kernel(AttnTask t) {
+constexpr int few_occupancy() {
+  return HDP == 256 ? 1 : (HDP == 64 && NT == 1 ? 3 : 2) - (WIDE || (sizeof(T) == 4 && HDP == 128 && NT == 1) ? 0 : 1);
+}
+
+template <class T, int HDP, int NT, bool WIDE>
+__global__ __launch_bounds__(kFewWaves * kWave, (few_occupancy<T, HDP, NT, WIDE>())) void attention_few_kernel(AttnTask t) {
   __shared__ FewLds<HDP, NT> lds;
   const int split = blockIdx.z / t.tiles;
   attention_few<T, HDP, NT, WIDE>(t, lds, blockIdx.x, blockIdx.y, split, blockIdx.z - split * t.tiles);
