@@ -12,8 +12,8 @@
 // scores form.  FP32 pages use v_mfma_f32_16x16x4_f32 on the values as they are.
 //
 // Measured (the kernel, then the join of its ranges): 12 requests of up to 32750 positions, 32 heads over 8 of 128, BF16 (1.17
-// GB): 218 + 5.0 us, 5.4 TB/s of the 5.9 that a read of memory reaches; 64 requests of up to 2047, 32 over 4 of 64, FP16
-// (103 MB): 19.5 + 4.7 us; one FP32 request of 2047: 6.5 + 3.6 us, bound by latency.  Registers for one more wave per SIMD: 26 -> 34 us at 64 requests.
+// GB): 220 + 4.8 us, 5.3 TB/s of the 5.9 that a read of memory reaches; 64 requests of up to 2047, 32 over 4 of 64, FP16
+// (103 MB): 19.7 + 4.1 us; one FP32 request of 2047: 6.7 + 3.7 us, bound by latency.  Registers for one more wave per SIMD: 26 -> 34 us at 64 requests.
 //
 // Masked positions: scores -inf, value rows zero.  A range whose sums come out infinite or NaN is computed again
 // by wave_attend, which reads only what each row sees.

@@ -10,11 +10,14 @@
 // products for FP16 keys and values, three for BF16.  FP32 tiles are scaled by powers of two and split into two
 // FP16 parts (three products), as they are staged or, for packed rows with enough work, by a kernel before.
 //
-// Bound by the matrix cores' rate under load: 9001 packed FP16 rows (508 GFLOP of attention, twice that in
-// products) 884 us, 1150 TFLOP/s of products where a large library product reaches 1187 (matrix units busy 58 to 60% of
-// the cycles, the clock falling from 1.82 to 1.52 GHz over three launches); 6001 FP32 rows 217 us, with the preparation, 8 to 11 in its traces; 500 rows after 8111 positions
-// of FP16 pages 150 us with the join.  Six products of three BF16 parts took 350 us for the 6001 FP32 rows; tiles
-// through registers instead of LDS-DMA 941 us for the 9001 (868 when first changed); sums taken in turn made no difference.
+// Bound by the matrix cores and, beside them, the vector instructions: 9001 packed FP16 rows (508 GFLOP of attention, twice that in
+// products) 873 us, 1165 TFLOP/s of products.  The matrix units are busy 61% of the cycles (70% in a large library product, which
+// reaches 1187) and the other vector instructions' issue takes 33% (11%): the two hardly overlap.  The clock falls from 1.8 to
+// 1.5 GHz over a few launches of either.  6001 FP32 rows 220 us, with the preparation, 10 to 12 in its traces; 500 rows after 8111 positions of FP16 pages
+// 151 us with the join, after 8000 of FP32 pages 155 (hd 64) and 318 (hd 128).  Six products of three BF16 parts took 350 us for the
+// 6001 FP32 rows; tiles through registers instead of LDS-DMA 941 us for the 9001 (868 when first changed); sums taken in turn made
+// no difference.  Looking for dims that FP16 tiles would lose costs FP32 pages up to 5% (32 rows after 8000, hd 128: 58 -> 61 us); flags of
+// every row's dims instead of the first rows' took 3 to 26%.
 //
 // Masked positions: scores -inf; rows past the last position or without a page are staged as zeros.  Pairs whose
 // sums come out infinite or NaN are computed again by wave_attend, which reads only what each row sees.

@@ -10,7 +10,7 @@ namespace {
 // the attention kernel takes them from the rows themselves.  Three products (high high, high low, low high) serve
 // FP32, two serve BF16, where its rows as they are take three.  The tile is written
 // as the kernel's LDS holds it: planes of K, planes of V.
-// Read and written once, in one pass: bound by memory and the launch (6001 rows of 4 heads of 64, 12 + 12 MB: 8 to 11 us).
+// Read and written once, in one pass: bound by memory and the launch (6001 rows of 4 heads of 64, 12 + 12 MB: 10 to 12 us).
 template <class T, int HDP>
 __global__ __launch_bounds__(kTileThreads) void attention_prepare_kernel(PrepareArgs a) {
   using Sh = TileShape<T, HDP, kPrepared>;

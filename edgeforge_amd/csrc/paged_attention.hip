@@ -88,13 +88,18 @@ PagedPlan plan_paged(size_t H, size_t KV, size_t hd, int qtype, size_t n_seqs, s
 // Whether packed FP32 and BF16 rows go through the prepared tiles: FP32 rows scaled and split
 // once instead of by every workgroup, BF16 two products for three; one more launch and pass.  By the
 // work, rows times rows of a prompt on average; us from the rows / prepared, 32 heads over 4 of 64 and over 8 of 128:
-//   FP32, 64:   100 rows 11.2 / 12.8, 200 rows 16.0 / 15.3, 333 of 9 prompts 11.5 / 13.8, 500 rows 28.0 / 23.2, 1000 of 8
-//               25.6 / 23.6, 2000 of 20 25.4 / 25.8, 2000 rows 95.3 / 73.0
-//   FP32, 128:  100 rows 18.6 / 16.5, 333 of 9 20.8 / 18.7, 500 rows 60.6 / 37.4, 2000 of 20 54.7 / 40.3
-//   FP32, 80 (12 heads over 4):  64 rows 10.9 / 12.6, 128 rows 15.9 / 15.0, 256 of 4 23.8 / 19.4
-//   FP32, 256 (8 over 4):  64 rows 28.8 / 26.7, 128 rows 41.8 / 33.8
-//   BF16, 64:   1000 rows 30.2 / 32.5, 1500 of 3 37 / 40, 2000 rows 61.5 / 59.1, 6000 of 4 181 / 144, 9000 rows 804 / 623
-//   BF16, 128:  1000 rows 46 / 57, 2000 rows 102 / 105, 3000 rows 188 / 157, 9000 rows 1443 / 1170
+//   FP32, 64:   100 rows 11.3 / 13.4, 200 rows 16.1 / 16.0, 333 of 9 prompts 11.6 / 14.2, 500 rows 28.3 / 24.1, 1000 of 8
+//               23.3 / 22.8, 2000 of 20 32.1 / 31.7, 2000 rows 96.9 / 76.2
+//   FP32, 128:  64 rows 15.0 / 15.3, 100 rows 18.8 / 17.0, 333 of 9 22.3 / 20.3, 500 rows 59.7 / 38.0, 2000 of 20 70.4 / 52.7
+//   FP32, 80 (12 heads over 4):  64 rows 10.9 / 13.1, 128 rows 16.0 / 15.7, 256 of 4 17.7 / 16.8
+//   FP32, 256 (8 over 4):  32 rows 19.7 / 20.8, 64 rows 29.6 / 27.7, 128 rows 42.9 / 35.4
+//   FP32, as many KV heads:  16 of 64, 200 rows 16.5 / 16.8, 500 28.0 / 24.7, 6000 297 / 235;  8 of 128, 200 29.8 / 22.3, 6000 630 / 329
+//   BF16, 64:   1000 rows 30.4 / 31.3, 1500 of 3 37.1 / 37.1, 2000 rows 60.1 / 56.6, 6000 of 4 168 / 137, 9000 rows 796 / 615
+//   BF16, 128:  1000 rows 46.6 / 54.6, 2000 rows 101 / 101, 3000 rows 187 / 159, 9000 rows 1438 / 1169
+//   BF16, as many KV heads:  16 of 64, 1000 rows 29.1 / 31.4, 6000 215 / 176;  8 of 128, 1000 43.6 / 51.9, 6000 250 / 242
+// The work alone does not know how many workgroups share a tile, nor how full the GPU is: it takes the slower way for many short prompts (FP32,
+// 128, 1000 rows of 50: 24.0 / 31.3) and, up to 20% slower, for middle lengths of as many KV heads (FP32, 16 of 64, 6000 of 30:
+// 48.5 / 56.1; BF16, 8 of 128, 3000 rows: 116 / 131) or of several BF16 prompts (64, 9000 of 20: 110 / 96).
 // EF_HIP_PACKED_ATTENTION=rows|prepared takes one or the other (tests).
 bool prepares(size_t hd, int qtype, size_t n_seqs, size_t max_rows) {
   if (qtype == EF_QTYPE_F16 || max_rows == 0) return false;

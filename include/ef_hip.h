@@ -346,7 +346,8 @@ typedef struct {
  * the free pages' numbers, the last one taken first; the array has room for n_pages.
  *  - The pages of ended requests (table entries in [0, n_pages)) are put on top of the free ones, in
  *    order; their table rows keep their entries, which no length reaches any more.
- *  - Growing requests take pages from the top, in order, into their table rows.
+ *  - Growing requests take pages from the top, in order, into their table rows.  (A page in two requests' rows would be
+ *    given back twice and taken twice: pages that requests share are the caller's to plan.)
  *  - row_start_dev[n_seqs + 1] gets the first row of each request (row_start_dev[n_seqs]: how many),
  *    pos_dev / slot_dev[max_rows] each row's position and slot (page * page_size + offset; position
  *    0 and slot -1 behind the last row), kv_len_dev[n_seqs] the positions after the step (0 for
@@ -384,9 +385,16 @@ int ef_hip_rope_append(const float* q_dev, size_t ldq, float* q_out_dev, size_t 
  *   out = sum_j softmax_j(scale * q . k_j) v_j,  query head h over KV head h / (heads / KV).
  * A page number outside [0, n_pages) is no page: its positions take no part.  A row that sees nothing
  * gets zeros, as one whose scores are all -inf does.  Rows in front of row_start_dev[0] (some of a
- * batch's requests, by pointers into the plan) and behind row_start_dev[n_seqs] stay as they were.  Infinite or NaN keys and values
- * stay with the rows that see them.  q / out are FP32 rows [..][heads * hd] with strides ldq / ldo.
- * Everything is held in 32 bits or more; results are the same on every call.
+ * batch's requests, by pointers into the plan) and behind row_start_dev[n_seqs] stay as they were.  Infinite or
+ * NaN keys and values stay with the rows that see them.  q / out are FP32 rows [..][heads * hd] with strides
+ * ldq / ldo.  Results are the same on every call with the same bounds.
+ * Sums, maxima and results are held in 32 bits or more.  What the matrix products take is
+ *  - all of it with BF16 pages, and with FP32 pages where max_new rows are at most 64 (row, head) pairs of a KV head;
+ *  - 22 bits of queries and weights with FP16 pages, and of FP32 keys and values too where there are more (two halves
+ *    each): never less than 2^-39 of a row's largest query, 2^-38 of its largest weight, and, of a key or value, 2^-24 of
+ *    (its row's largest) (its dim's largest) / (the largest) among the 32 or 64 positions of its tile.  A tile that
+ *    would lose more (rows or dims 2^11 and more apart), or whose values are 2^12 and more from the others' in size, is
+ *    taken position by position in FP32, which is right but slow.
  * table_ld pages hold at most 2^31 - 1024 positions.
  * The bounds are the host's: max_rows rows in q and out, max_new rows of one request, max_kv positions
  * of one request.  max_rows is kept to (rows behind it are neither read nor written; those of the same request
@@ -407,7 +415,8 @@ int ef_hip_paged_attention(const float* q_dev, size_t ldq, float* out_dev, size_
 /* Causal attention over whole prompts packed one after another, without a cache: rows row_start_dev[r] ..
  * row_start_dev[r + 1] of q, k and v are prompt r, whose row i sees its rows 0 .. i.  k / v rows hold [KV * hd]
  * values of `qtype` (F32, F16 or BF16) with strides ldk / ldv in values; the rest as in
- * ef_hip_paged_attention.  Strides and addresses at multiples of 16 bytes, hd a multiple of 8 up to 256. */
+ * ef_hip_paged_attention (FP32 keys and values always as with many rows; BF16 ones, exactly or as halves of the same
+ * bounds).  Strides and addresses at multiples of 16 bytes, hd a multiple of 8 up to 256. */
 size_t ef_hip_packed_attention_workspace_bytes(size_t heads, size_t KV, size_t hd, int qtype, size_t n_seqs,
                                                size_t max_rows);
 int ef_hip_packed_attention(const float* q_dev, size_t ldq, const void* k_dev, size_t ldk, const void* v_dev, size_t ldv,
