@@ -129,7 +129,7 @@ constexpr int kNoTile = INT32_MIN, kAnyScale = INT32_MAX;
 
 // A tile's exponents, and what the largest value of each of its dims has to reach, from the bits of the largest
 // magnitude of its keys and of its values and of the smallest among its rows' largest magnitudes (rows of zeros left
-// out).  Keys are brought to 2^14 .. 2^15 (c2 takes each tile's scale back), values to 2^11 .. 2^15, so that neighbouring tiles
+// out).  Keys are brought to 2^14 .. 2^15 (c2 takes each tile's scale back), values to 2^13 .. 2^15, so that neighbouring tiles
 // mostly share a scale and the sums keep theirs.
 //   What the halves drop of a value is 2^-25 at most or 2^-22 of it: below 2^-24 of (its row's largest) (its dim's largest) /
 //   (the tile's largest) as long as that is 1/2 or more for each row and dim.  The tile's largest is below 2^(M + 1), the rows' are
@@ -144,7 +144,7 @@ __device__ __forceinline__ TileScales tile_scales(uint32_t k_most, uint32_t k_le
   };
   const int lk = lead(k_most, k_least), lv = lead(v_most, v_least);
   const int ek = k_most == 0 ? kAnyScale : 14 + 127 - static_cast<int>(k_most >> 23);
-  const int ev = v_most == 0 ? kAnyScale : (14 + 127 - static_cast<int>(v_most >> 23)) & ~3;
+  const int ev = v_most == 0 ? kAnyScale : (14 + 127 - static_cast<int>(v_most >> 23)) & ~1;
   const bool marked = k_most >= 0x7F800000u || v_most >= 0x7F800000u || max(lk, lv) > 14;  // 2^15: no dim would reach it
   return {marked ? int2{kNoTile, kNoTile} : int2{ek, ev}, ldexpf(1.0f, lk - ek), ldexpf(1.0f, lv - ev)};
 }

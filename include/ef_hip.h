@@ -393,8 +393,8 @@ int ef_hip_rope_append(const float* q_dev, size_t ldq, float* q_out_dev, size_t 
  *  - 22 bits of queries and weights with FP16 pages, and of FP32 keys and values too where there are more (two halves
  *    each): never less than 2^-39 of a row's largest query, 2^-38 of its largest weight, and, of a key or value, 2^-24 of
  *    (its row's largest) (its dim's largest) / (the largest) among the 32 or 64 positions of its tile.  A tile that
- *    would lose more (rows or dims 2^11 and more apart), or whose values are 2^12 and more from the others' in size, is
- *    taken position by position in FP32, which is right but slow.
+ *    would lose more (rows or dims 2^13 and more apart, or one value some 100 times all others), or whose values are 2^12
+ *    and more from the others' in size, is taken position by position in FP32, which is right but slow.
  * table_ld pages hold at most 2^31 - 1024 positions.
  * The bounds are the host's: max_rows rows in q and out, max_new rows of one request, max_kv positions
  * of one request.  max_rows is kept to (rows behind it are neither read nor written; those of the same request
